@@ -487,6 +487,33 @@ int bsp_matmul_use_tcgen05(int enable);
  */
 int bsp_matmul_prefers_tcgen05(int op, int block, int Z, int free_size, int trans_s, const int32_t* meta_hdr, int* prefers);
 
+/* ------------------------------------------------------------------------ */
+/* Rotary positions (device)                                                */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * Pairs of channels of q and k turned by the angle of their token's position
+ * (no counterpart in the reference):
+ *   y0 = x0 cos t - x1 sin t,  y1 = x1 cos t + x0 sin t,
+ * with -t when `inverse` is set, which is the gradient.  q [Z, Hq, L, D] and k
+ * [Z, Hk, L, D] with unit stride on D and z / h / l strides of their own, outputs
+ * too; an operand is absent when its number of heads is 0; an output may be its
+ * operand (same strides).  Pair i is channels (i, pairs + i), or (2i, 2i + 1) with
+ * `interleaved` (strides even, bases aligned to two elements); channels from
+ * 2 * pairs on are copied.  D at most 256.
+ * table      DEVICE [2, pairs]: what one position adds to a pair's angle, as a
+ *            64-bit two's complement fraction of a whole turn, and its axis.
+ * positions  DEVICE, pos_bytes (4 or 8) each, element (axis, z, l) at
+ *            axis*p_sa + z*p_sz + l*p_sl; pos_bytes 0: l itself (one axis).
+ */
+int bsp_rotary(const void* q, void* q_out, int Hq, int64_t q_sz, int64_t q_sh, int64_t q_sl,
+               int64_t qo_sz, int64_t qo_sh, int64_t qo_sl,
+               const void* k, void* k_out, int Hk, int64_t k_sz, int64_t k_sh, int64_t k_sl,
+               int64_t ko_sz, int64_t ko_sh, int64_t ko_sl,
+               int dtype, int Z, int L, int D, int pairs, int interleaved,
+               const int64_t* table, int axes, const void* positions, int pos_bytes,
+               int64_t p_sa, int64_t p_sz, int64_t p_sl, int inverse, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

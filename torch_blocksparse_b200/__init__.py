@@ -9,7 +9,8 @@ from .matmul import MatMul, Linear
 from .attention import DeepSpeedSparseSelfAttention, SparseSelfAttention, SparsityConfig
 from .mha import MultiheadAttention, replace_mha, make_layout
 from .host import HostAttention
+from .rotary import Rotary
 from . import layouts
 
 __all__ = ['Softmax', 'MatMul', 'Linear', 'DeepSpeedSparseSelfAttention', 'SparseSelfAttention',
-           'SparsityConfig', 'MultiheadAttention', 'replace_mha', 'make_layout', 'HostAttention', 'layouts']
+           'SparsityConfig', 'MultiheadAttention', 'replace_mha', 'make_layout', 'HostAttention', 'Rotary', 'layouts']

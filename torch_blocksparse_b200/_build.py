@@ -19,7 +19,7 @@ PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 SRC_DIR = os.path.join(PKG_DIR, 'csrc')
 OBJ_DIR = os.path.join(PKG_DIR, 'build')
 LIB_PATH = os.path.join(PKG_DIR, 'libbsp_b200.so')
-OPS_SRC = os.path.join(SRC_DIR, 'torch', 'ops.cpp')
+OPS_DIR = os.path.join(SRC_DIR, 'torch')
 OPS_PATH = os.path.join(PKG_DIR, '_ops.so')
 INCLUDE_DIR = os.path.join(os.path.dirname(PKG_DIR), 'include')
 
@@ -54,8 +54,12 @@ def needs_build():
     return _mtime(LIB_PATH) < newest_src
 
 
+def _ops_files(*ends):
+    return sorted(os.path.join(OPS_DIR, f) for f in os.listdir(OPS_DIR) if f.endswith(ends))
+
+
 def _ops_need_build():
-    return _mtime(OPS_PATH) < max(_mtime(OPS_SRC), _mtime(os.path.join(INCLUDE_DIR, 'bsp.h')))
+    return _mtime(OPS_PATH) < max(_mtime(f) for f in _ops_files('.cpp', '.h') + [os.path.join(INCLUDE_DIR, 'bsp.h')])
 
 
 def _run(cmd, verbose):
@@ -65,22 +69,41 @@ def _run(cmd, verbose):
     return r.returncode == 0
 
 
-def _build_ops(verbose=False):
+def _build_ops(force=False, verbose=False):
     """Compile the torch module; it finds libbsp_b200.so next to itself."""
     import torch
     root = os.path.dirname(torch.__file__)
     cuda = os.path.dirname(os.path.dirname(_nvcc())) if os.path.isabs(_nvcc()) else '/usr/local/cuda'
     inc = [os.path.join(root, 'include'), os.path.join(root, 'include', 'torch', 'csrc', 'api', 'include'),
            os.path.join(cuda, 'include'), sysconfig.get_paths()['include'], INCLUDE_DIR]
+    flags = (['-O3', '-std=c++17', '-fPIC', '-fvisibility=hidden',
+              '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi(), '-DTORCH_EXTENSION_NAME=_ops']
+             + [x for d in inc for x in ('-isystem' if d != INCLUDE_DIR else '-I', d)])
+    newest_hdr = max(_mtime(f) for f in _ops_files('.h') + [os.path.join(INCLUDE_DIR, 'bsp.h')])
+    os.makedirs(OBJ_DIR, exist_ok=True)
+    jobs, objs = [], []
+    for src in _ops_files('.cpp'):
+        obj = os.path.join(OBJ_DIR, 'torch_' + os.path.basename(src) + '.o')
+        objs.append(obj)
+        if force or _mtime(obj) < max(_mtime(src), newest_hdr):
+            jobs.append((src, obj))
+
+    def compile_one(job):
+        src, obj = job
+        tmp = obj + '.%d' % os.getpid()
+        if not _run(['g++'] + flags + ['-c', src, '-o', tmp], verbose):
+            raise RuntimeError('compiling %s failed' % src)
+        os.replace(tmp, obj)
+
+    with ThreadPoolExecutor(max_workers=max(1, len(jobs))) as ex:
+        list(ex.map(compile_one, jobs))
     tmp = OPS_PATH + '.%d' % os.getpid()
-    cmd = (['g++', '-O3', '-std=c++17', '-fPIC', '-shared', '-fvisibility=hidden',
-            '-D_GLIBCXX_USE_CXX11_ABI=%d' % torch.compiled_with_cxx11_abi(), '-DTORCH_EXTENSION_NAME=_ops']
-           + [x for d in inc for x in ('-isystem' if d != INCLUDE_DIR else '-I', d)] + [OPS_SRC, '-o', tmp]
+    cmd = (['g++', '-shared'] + objs + ['-o', tmp]
            + ['-L' + os.path.join(root, 'lib'), '-lc10', '-lc10_cuda', '-ltorch_cpu', '-ltorch_python', '-ltorch',
               '-L' + os.path.join(cuda, 'lib64'), '-lcudart_static', '-ldl', '-lrt', '-lpthread',
               '-L' + PKG_DIR, '-l:' + os.path.basename(LIB_PATH), '-Wl,-rpath,$ORIGIN'])
     if not _run(cmd, verbose):
-        raise RuntimeError('compiling %s failed' % OPS_SRC)
+        raise RuntimeError('linking %s failed' % OPS_PATH)
     os.replace(tmp, OPS_PATH)
 
 
@@ -90,7 +113,7 @@ def build(force=False, verbose=False):
     if force or needs_build():
         _build_lib(force, verbose)
     if force or _ops_need_build():
-        _build_ops(verbose)
+        _build_ops(force, verbose)
     return LIB_PATH
 
 

@@ -11,70 +11,17 @@
 //   MatMul      torch_blocksparse/matmul.py:299-364, 460-552, 558-606
 //   Softmax     torch_blocksparse/softmax.py:253-326 (in place; rpe and masks get no gradient)
 //   Attention   torch_blocksparse/deepspeedsparseselfattention.py:135-166
-#include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/utils/pybind.h>
-#include <torch/types.h>
 #include <ATen/ops/constant_pad_nd.h>
-#include <ATen/ops/empty.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <c10/cuda/CUDAStream.h>
-#include <cuda_runtime_api.h>
 
-#include "bsp.h"
+#include "host.h"
+
+void bind_serving(pybind11::module_& m);   // serving.cpp
 
 namespace {
 
-using at::Tensor;
-using OptTensor = std::optional<Tensor>;
-using torch::autograd::AutogradContext;
-using torch::autograd::variable_list;
+using namespace bsp_host;
 
 constexpr int kMaxSoftmaxRow = 32768;
-
-// ---- errors and arguments ----------------------------------------------------------------------
-[[noreturn]] void raise_status(int rc) {
-  const char* msg = bsp_last_error();
-  switch (rc) {
-    case BSP_ERR_INVALID: TORCH_CHECK_VALUE(false, msg);
-    case BSP_ERR_UNSUPPORTED: TORCH_CHECK_NOT_IMPLEMENTED(false, msg);
-    default: TORCH_CHECK(false, msg);
-  }
-  TORCH_CHECK(false, msg);
-}
-void check(int rc) { if (rc != BSP_OK) raise_status(rc); }
-
-int dtype_code(const Tensor& t) {
-  switch (t.scalar_type()) {
-    case at::kFloat: return BSP_F32;
-    case at::kHalf: return BSP_F16;
-    case at::kBFloat16: return BSP_BF16;
-    default: TORCH_CHECK_VALUE(false, "unsupported dtype ", t.scalar_type(), " (float32, float16 and bfloat16 are)");
-  }
-}
-
-void require_cuda(const Tensor& t) {
-  TORCH_CHECK(t.is_cuda(), "torch_blocksparse_b200 runs on CUDA tensors only (got a ", t.device(), " tensor)");
-}
-
-// Everything a call reads has to lie on one device, and a pointer has to be of the type it is read as.
-void require_same(const Tensor& t, const Tensor& ref, const char* what) {
-  TORCH_CHECK(t.device() == ref.device(), what, " is on ", t.device(), ", the call runs on ", ref.device());
-  TORCH_CHECK_VALUE(t.scalar_type() == ref.scalar_type(), what, " must be ", ref.scalar_type(), " (got ", t.scalar_type(), ")");
-}
-
-// Whether a call on these tensors goes through autograd: one of them needs a gradient (a bias or a
-// mask too, although it receives none: the result can then be differentiated), or carries a
-// forward-mode tangent, which the functions below refuse (passing them by would drop it silently).
-bool needs_grad(const Tensor& t) { return t.requires_grad(); }
-bool needs_grad(const OptTensor& t) { return t && t->requires_grad(); }
-bool has_tangent(const Tensor& t) { return t._fw_grad(0).defined(); }
-bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
-template <typename... Ts> bool recorded(const Ts&... t) {
-  return (at::GradMode::is_enabled() && (needs_grad(t) || ...)) || (has_tangent(t) || ...);
-}
-void* stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
-int64_t vec_of(const Tensor& t) { return 16 / static_cast<int64_t>(t.element_size()); }
-bool aligned16(const Tensor& t) { return (reinterpret_cast<uintptr_t>(t.const_data_ptr()) & 15) == 0; }
 
 // Wall time of one launch (bench=True), in seconds, and what the reference calls it.
 struct Times : torch::CustomClassHolder {
@@ -663,4 +610,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::make_tuple(o.q, o.k, o.v, o.rpe, o.kpm, o.am);
   });
   m.def("attention_gradient", &rows_for);
+  bind_serving(m);
 }

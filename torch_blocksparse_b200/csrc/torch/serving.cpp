@@ -1,0 +1,162 @@
+// Host path of rotary positions, the 4-bit key / value cache and attention over it.
+#include <ATen/ops/empty_like.h>
+
+#include "host.h"
+
+namespace {
+
+using namespace bsp_host;
+
+// ---- rotary positions --------------------------------------------------------------------------
+struct RotaryOp : torch::CustomClassHolder {
+  Tensor table;                            // [2, pairs] int64 on one device: turns, axes
+  int64_t head_dim, axes;
+  bool interleaved;
+};
+
+struct Positions {
+  const void* at = nullptr;
+  int bytes = 0;
+  int64_t sa = 0, sz = 0, sl = 0;
+};
+
+// [L], [axes, L] or [axes, Z, L] whole numbers; dimensions of size 1 are shared by the batch.
+Positions positions_of(const OptTensor& pos, const RotaryOp& p, const Tensor& q) {
+  Positions r;
+  const int64_t Z = q.size(0), L = q.size(2);
+  if (!pos) {
+    TORCH_CHECK_VALUE(p.axes == 1, "rotary: positions are needed for ", p.axes, " axes");
+    return r;
+  }
+  TORCH_CHECK(pos->device() == q.device(), "rotary: the positions are on ", pos->device(), ", the call runs on ", q.device());
+  TORCH_CHECK_VALUE(pos->scalar_type() == at::kInt || pos->scalar_type() == at::kLong,
+                    "rotary: positions must be int32 or int64 (got ", pos->scalar_type(), ")");
+  const int64_t d = pos->dim();
+  TORCH_CHECK_VALUE(d >= 1 && d <= 3 && pos->size(d - 1) == L && (d < 2 ? p.axes == 1 : pos->size(0) == p.axes) &&
+                        (d < 3 || pos->size(1) == Z || pos->size(1) == 1),
+                    "rotary: positions must be [", p.axes, ", ", Z, ", ", L, "], [", p.axes, ", ", L, "]",
+                    p.axes == 1 ? " or, for one axis, [L]" : "", " (got ", pos->sizes(), ")");
+  r.at = pos->const_data_ptr();
+  r.bytes = static_cast<int>(pos->element_size());
+  r.sl = pos->stride(d - 1);
+  if (d > 1) r.sa = pos->stride(0);
+  if (d == 3 && pos->size(1) > 1) r.sz = pos->stride(1);
+  return r;
+}
+
+// Rows with a unit stride; neighbouring pairs also on a boundary of a pair's size.
+Tensor rotary_rows(const Tensor& x, bool pairs) {
+  const int64_t even = pairs ? 2 : 1;
+  bool ok = x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.const_data_ptr()) % (even * x.element_size()) == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (x.size(i) == 1 || x.stride(i) % even == 0);
+  return ok ? x : x.clone(at::MemoryFormat::Contiguous);
+}
+// The result, in the memory order of x.
+Tensor rotary_out(const Tensor& x) {
+  Tensor y = at::empty_like(x);
+  return y.stride(3) == 1 ? y : at::empty(x.sizes(), x.options());
+}
+
+std::pair<Tensor, Tensor> rotary(const RotaryOp& p, const OptTensor& q0, const OptTensor& k0, const OptTensor& pos, bool inverse) {
+  const Tensor& any = q0 ? *q0 : *k0;
+  const c10::cuda::CUDAGuard guard(any.device());
+  const Positions at = positions_of(pos, p, any);
+  Tensor x[2], y[2];
+  int64_t s[2][6] = {};
+  for (int i = 0; i < 2; ++i) {
+    const OptTensor& t = i ? k0 : q0;
+    if (!t) continue;
+    x[i] = rotary_rows(*t, p.interleaved);
+    y[i] = rotary_out(x[i]);
+    for (int j = 0; j < 3; ++j) {
+      s[i][j] = x[i].stride(j);
+      s[i][3 + j] = y[i].stride(j);
+    }
+  }
+  auto in = [&](int i) { return x[i].defined() ? x[i].const_data_ptr() : nullptr; };
+  auto out = [&](int i) { return y[i].defined() ? y[i].mutable_data_ptr() : nullptr; };
+  auto heads = [&](int i) { return x[i].defined() ? x[i].size(1) : 0; };
+  check(bsp_rotary(in(0), out(0), heads(0), s[0][0], s[0][1], s[0][2], s[0][3], s[0][4], s[0][5], in(1), out(1), heads(1), s[1][0],
+                   s[1][1], s[1][2], s[1][3], s[1][4], s[1][5], dtype_code(any), any.size(0), any.size(2), any.size(3),
+                   p.table.size(1), p.interleaved, p.table.const_data_ptr<int64_t>(), p.axes, at.at, at.bytes, at.sa, at.sz, at.sl,
+                   inverse, stream_of(any)));
+  return {y[0], y[1]};
+}
+
+std::pair<Tensor, Tensor> rotary_recorded(const c10::intrusive_ptr<RotaryOp>& p, const OptTensor& q, const OptTensor& k,
+                                          const OptTensor& pos, bool inverse);
+
+struct RotaryFn : torch::autograd::Function<RotaryFn> {
+  static variable_list forward(AutogradContext* ctx, const c10::intrusive_ptr<RotaryOp>& p, const OptTensor& q, const OptTensor& k,
+                               const OptTensor& pos, bool inverse) {
+    ctx->set_materialize_grads(false);
+    ctx->saved_data["p"] = c10::IValue::make_capsule(p);
+    ctx->saved_data["inverse"] = inverse;
+    ctx->saved_data["q"] = q.has_value();
+    if (pos) ctx->save_for_backward({*pos});
+    auto [yq, yk] = rotary(*p, q, k, pos, inverse);
+    if (!q) return {yk};
+    return k ? variable_list{yq, yk} : variable_list{yq};
+  }
+  // The turn back; a gradient of its own, so that it can be differentiated again.
+  static variable_list backward(AutogradContext* ctx, const variable_list& grads) {
+    const auto p = c10::static_intrusive_pointer_cast<RotaryOp>(ctx->saved_data["p"].toCapsule());
+    const variable_list saved = ctx->get_saved_variables();
+    const OptTensor pos = saved.empty() ? OptTensor() : OptTensor(saved[0]);
+    const bool has_q = ctx->saved_data["q"].toBool();
+    OptTensor dq, dk;
+    if (has_q && grads[0].defined()) dq = grads[0];
+    const size_t at = has_q ? 1 : 0;
+    if (grads.size() > at && grads[at].defined()) dk = grads[at];
+    variable_list out(5);
+    if (!dq && !dk) return out;
+    auto [q, k] = rotary_recorded(p, dq, dk, pos, !ctx->saved_data["inverse"].toBool());
+    out[1] = q;
+    out[2] = k;
+    return out;
+  }
+};
+
+std::pair<Tensor, Tensor> rotary_recorded(const c10::intrusive_ptr<RotaryOp>& p, const OptTensor& q, const OptTensor& k,
+                                          const OptTensor& pos, bool inverse) {
+  auto is = [](const OptTensor& t) { return t && recorded(*t); };
+  if (!is(q) && !is(k)) return rotary(*p, q, k, pos, inverse);
+  const variable_list y = RotaryFn::apply(p, q, k, pos, inverse);
+  if (!q) return {Tensor(), y[0]};
+  return {y[0], k ? y[1] : Tensor()};
+}
+
+void check_rotary(const RotaryOp& p, const Tensor& x, const char* what) {
+  TORCH_CHECK_VALUE(x.dim() == 4 && x.size(3) == p.head_dim, "rotary: ", what, " must be [Z, H, L, ", p.head_dim, "] (got ", x.sizes(), ")");
+  require_cuda(x);
+  dtype_code(x);
+  TORCH_CHECK(x.device() == p.table.device(), "rotary: ", what, " is on ", x.device(), ", the call runs on ", p.table.device());
+}
+
+std::pair<Tensor, OptTensor> rotary_call(const c10::intrusive_ptr<RotaryOp>& p, const Tensor& q, const OptTensor& k,
+                                         const OptTensor& pos) {
+  check_rotary(*p, q, "the query");
+  if (k) {
+    check_rotary(*p, *k, "the key");
+    require_same(*k, q, "rotary: the key");
+    TORCH_CHECK_VALUE(k->size(0) == q.size(0) && k->size(2) == q.size(2), "rotary: query ", q.sizes(), " and key ", k->sizes(),
+                      " differ in batch or length");
+  }
+  auto [yq, yk] = rotary_recorded(p, q, k, pos, false);
+  return {yq, yk.defined() ? OptTensor(yk) : OptTensor()};
+}
+
+}  // namespace
+
+void bind_serving(pybind11::module_& m) {
+  namespace py = pybind11;
+  py::class_<RotaryOp, c10::intrusive_ptr<RotaryOp>>(m, "RotaryOp")
+      .def(py::init([](Tensor table, int64_t head_dim, int64_t axes, bool interleaved) {
+        auto p = c10::make_intrusive<RotaryOp>();
+        p->table = table; p->head_dim = head_dim; p->axes = axes; p->interleaved = interleaved;
+        return p;
+      }))
+      .def("__call__", &rotary_call, py::call_guard<py::gil_scoped_release>())
+      .def("one", [](const c10::intrusive_ptr<RotaryOp>& p, const Tensor& x, const OptTensor& pos) { return rotary_call(p, x, {}, pos).first; },
+           py::call_guard<py::gil_scoped_release>());
+}

@@ -15,6 +15,9 @@ attention core between them -- q scaled by head_dim^-1/2, sparse scores, masked
 softmax without further scale, product with v (attention.py:127, 190-198) -- runs
 in the fused kernel.  As in the reference only self-attention without dropout is
 supported and no attention weights are returned.
+
+Beyond the reference: `rotary` (a Rotary for this module's head dimension) turns queries and keys by
+forward's `positions` (see Rotary; None: 0, 1, .. L - 1) before their product.
 """
 import torch
 import torch.nn as nn
@@ -32,8 +35,11 @@ def make_layout(num_heads, num_blocks, mode, block_stride, unidirectional, numve
 
 class MultiheadAttention(nn.modules.activation.MultiheadAttention):
 
+    rotary = None                      # (of the class: modules saved before there were positions have none)
+
     def __init__(self, embed_dim, num_heads, layout, block, dropout=0., bias=True, add_bias_kv=False,
-                 add_zero_attn=False, kdim=None, vdim=None, key_padding_mask_mode='add', attn_mask_mode='mul'):
+                 add_zero_attn=False, kdim=None, vdim=None, key_padding_mask_mode='add', attn_mask_mode='mul',
+                 rotary=None):
         if dropout != 0:
             raise NotImplementedError('dropout is not supported for now')
         super().__init__(embed_dim, num_heads, dropout, bias, add_bias_kv, add_zero_attn, kdim, vdim)
@@ -43,12 +49,16 @@ class MultiheadAttention(nn.modules.activation.MultiheadAttention):
         self.block = block
         self.key_padding_mask_mode = key_padding_mask_mode
         self.attn_mask_mode = attn_mask_mode
+        if rotary is not None:
+            if rotary.head_dim != embed_dim // num_heads:
+                raise ValueError(f'rotary positions for heads of {rotary.head_dim} channels, not of {embed_dim // num_heads}')
+            self.rotary = rotary
         # the core: scores are not scaled again (q is pre-scaled), masks follow the softmax op's modes
         self.core = DeepSpeedSparseSelfAttention(layout=layout, block=block,
                                                  key_padding_mask_mode=key_padding_mask_mode,
                                                  attn_mask_mode=attn_mask_mode)
 
-    def forward(self, query, key, value, key_padding_mask=None, need_weights=True, attn_mask=None):
+    def forward(self, query, key, value, key_padding_mask=None, need_weights=True, attn_mask=None, positions=None):
         if query.shape != key.shape or key.shape != value.shape:
             raise NotImplementedError('only self-attention is supported for now')
         tgt_len, bsz, embed_dim = query.shape
@@ -76,7 +86,12 @@ class MultiheadAttention(nn.modules.activation.MultiheadAttention):
         # batch / head / row strides, so the projections are used where they lie, and the result
         # is written in [L, B, E] order by the kernel (no transposed copies on the way in or out)
         to_heads = lambda t: t.view(tgt_len, bsz, H, head_dim).permute(1, 2, 0, 3)
-        out = self.core.attend(to_heads(q), to_heads(k), to_heads(v), 1.0, None, key_padding_mask, attn_mask,
+        q, k = to_heads(q), to_heads(k)
+        if self.rotary is not None:
+            q, k = self.rotary(q, k, positions)
+        elif positions is not None:
+            raise ValueError('positions are given, but the module was built without rotary=')
+        out = self.core.attend(q, k, to_heads(v), 1.0, None, key_padding_mask, attn_mask,
                                seq_first_out=True)
         out = out.permute(2, 0, 1, 3).reshape(tgt_len, bsz, embed_dim)
         return F.linear(out, self.out_proj.weight, self.out_proj.bias), None
