@@ -514,6 +514,62 @@ int bsp_rotary(const void* q, void* q_out, int Hq, int64_t q_sz, int64_t q_sh, i
                const int64_t* table, int axes, const void* positions, int pos_bytes,
                int64_t p_sa, int64_t p_sz, int64_t p_sl, int inverse, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* 4-bit key / value cache (device)                                         */
+/* ------------------------------------------------------------------------ */
+
+/*
+ * A paged cache of keys and values (no counterpart in the reference).  For
+ * every token, head and 32 channels it holds s = bf16(max |x| / 7) and codes
+ * rint(x / s) in [-8, 7], and stands for s * code; where a channel is an infinity
+ * or a NaN, s is NaN.  D is 64 or 128.
+ * data       DEVICE, 16-byte aligned, num_pages * H * bsp_cache_page_bytes(page, D)
+ *            bytes in a private format; `page` tokens a page, a power of two from
+ *            16 to 1024.
+ * pages      DEVICE [Z, slots] with z-stride pages_sz: the page of a sequence's
+ *            tokens slot*page .. slot*page + page - 1; anything outside 0 ..
+ *            num_pages - 1 is no page.
+ * start      DEVICE [Z]: position of the call's first token in every sequence.
+ * count      DEVICE [Z] or NULL (T): how many of the T tokens there are.
+ * Every position, slot and page id is checked on the device; tokens without a
+ * place are not written, and read as zeros.
+ */
+int64_t bsp_cache_page_bytes(int page, int D);
+
+/*
+ * Quantises tokens 0 .. count - 1 of k and v [Z, H, T, D] (FP16 or BF16, unit
+ * stride on D) into positions start .. start + count - 1.  Nothing else in the
+ * cache is changed.  Two sequences of one call must not share a page that is written.
+ */
+int bsp_cache_write(const void* k, const void* v, int dtype, int Z, int H, int T, int D,
+                    int64_t k_sz, int64_t k_sh, int64_t k_st, int64_t v_sz, int64_t v_sh, int64_t v_st,
+                    void* data, int num_pages, int page, const int32_t* pages, int64_t pages_sz, int slots,
+                    const int32_t* start, const int32_t* count, void* stream);
+
+/*
+ * Positions start .. start + T - 1 of every sequence as k and v [Z, H, T, D] of any
+ * dtype (rows 16-byte aligned); zeros from token `count` on.
+ */
+int bsp_cache_read(void* k, void* v, int dtype, int Z, int H, int T, int D,
+                   int64_t k_sz, int64_t k_sh, int64_t k_st, int64_t v_sz, int64_t v_sh, int64_t v_st,
+                   const void* data, int num_pages, int page, const int32_t* pages, int64_t pages_sz, int slots,
+                   const int32_t* start, const int32_t* count, void* stream);
+
+/*
+ * Attention of the newest T tokens of every sequence over the cache: query t of
+ * sequence z stands at position lengths[z] - T + t (DEVICE [Z]) and sees the keys at
+ * positions up to its own that lie in the nonzero blocks of its block-row:
+ * o = softmax(scale * q K^T) V.  q, o [Z, Hq, T, D] (FP16 or BF16, unit stride
+ * on D); query head h reads head h / (Hq / Hk) of the cache.  meta: metadata
+ * of a square layout of 1 or Hk heads.  Queries that see nothing (positions below
+ * zero or behind the layout's last row, pages that are none) give zeros.
+ */
+int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D,
+                   int64_t q_sz, int64_t q_sh, int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st,
+                   const void* data, int num_pages, int page, const int32_t* pages, int64_t pages_sz, int slots,
+                   const int32_t* lengths, int block, const int32_t* meta_hdr, const int32_t* meta,
+                   float scale, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

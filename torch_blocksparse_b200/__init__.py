@@ -10,7 +10,9 @@ from .attention import DeepSpeedSparseSelfAttention, SparseSelfAttention, Sparsi
 from .mha import MultiheadAttention, replace_mha, make_layout
 from .host import HostAttention
 from .rotary import Rotary
+from .cache import KVCache
 from . import layouts
 
 __all__ = ['Softmax', 'MatMul', 'Linear', 'DeepSpeedSparseSelfAttention', 'SparseSelfAttention',
-           'SparsityConfig', 'MultiheadAttention', 'replace_mha', 'make_layout', 'HostAttention', 'Rotary', 'layouts']
+           'SparsityConfig', 'MultiheadAttention', 'replace_mha', 'make_layout', 'HostAttention', 'Rotary',
+           'KVCache', 'layouts']

@@ -26,6 +26,7 @@ _I32P = POINTER(c_int32)
 _IP = POINTER(c_int)
 _STRIDE3 = [c_int64, c_int64, c_int64]
 _MASKS = [c_void_p] + _STRIDE3 + [c_void_p, c_int64, c_int, c_void_p, c_int64, c_int]
+_CACHE = [c_void_p, c_int, c_int, c_void_p, c_int64, c_int]
 
 _SIGNATURES = {
     'bsp_last_error': (c_char_p, []),
@@ -70,6 +71,11 @@ _SIGNATURES = {
                            + _MASKS + [c_int, c_void_p]),
     'bsp_rotary': (c_int, [c_void_p, c_void_p, c_int] + [c_int64] * 6 + [c_void_p, c_void_p, c_int] + [c_int64] * 6
                    + [c_int] * 6 + [c_void_p, c_int, c_void_p, c_int] + [c_int64] * 3 + [c_int, c_void_p]),
+    'bsp_cache_page_bytes': (c_int64, [c_int, c_int]),
+    'bsp_cache_write': (c_int, [c_void_p, c_void_p] + [c_int] * 5 + [c_int64] * 6 + _CACHE + [c_void_p] * 3),
+    'bsp_cache_read': (c_int, [c_void_p, c_void_p] + [c_int] * 5 + [c_int64] * 6 + _CACHE + [c_void_p] * 3),
+    'bsp_cache_attn': (c_int, [c_void_p, c_void_p] + [c_int] * 6 + [c_int64] * 6 + _CACHE
+                       + [c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p]),
 }
 
 

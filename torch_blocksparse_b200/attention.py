@@ -46,7 +46,7 @@ class SparsityConfig:
 class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
 
     _op_cache = '_attn'
-    _op_attributes = frozenset(('block',))
+    _op_attributes = frozenset(('block', 'layout', 'sparsity_config'))
 
     @staticmethod
     def _make_layout(num_heads, num_blocks, mode, block_stride, attention, numverts, vertsize):
@@ -204,6 +204,36 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         w = softmax(w, scale=scaling, rpe=rpe, key_padding_mask=key_padding_mask, attn_mask=attn_mask,
                     key_padding_mask_mode=self.key_padding_mask_mode, attn_mask_mode=self.attn_mask_mode)
         return dsd_nn(w, value)
+
+
+    def decode(self, query, cache, pages, lengths, scale=None):
+        """Attention of the newest tokens of every sequence over a KVCache that holds their keys and values
+        already.  query [Z, heads, T, head_dim] (FP16 or BF16; heads a multiple of the cache's, neighbouring
+        ones share a head of it); pages int32 [Z, slots], the sequences' page table (see KVCache);
+        lengths int32 [Z], tokens of each sequence, the T new ones included.  Returns [Z, heads, T, head_dim].
+
+        Query t stands at position lengths[z] - T + t and sees the keys up to its own position that lie in
+        the nonzero blocks of its block-row: what forward() gives for that row under a causal
+        attn_mask.  The layout is the module's own, [heads of the cache or 1, ...], or its configuration's for
+        sequences as long as the page table; rows behind its end see nothing.  Positions below zero
+        (sequences shorter than T) and queries that see nothing give zeros.  scale: head_dim ** -0.5.
+
+        One kernel, without workspace, on the current stream of the cache's device; no gradient.  Lengths
+        and tables are read on the device, so that a captured call can be replayed as sequences grow."""
+        cache_op = cache._op()
+        key = ('decode', query.get_device(), cache.num_heads, None if self.layout is not None else pages.size(-1) * cache.page)
+        op = self._attn.get(key) or self._decode_op(key, cache, query.device)
+        return op(query, cache_op, pages, lengths, float(query.size(-1)) ** -0.5 if scale is None else float(scale))
+
+    def _decode_op(self, key, cache, device):
+        layout = self.layout
+        if layout is None:
+            layout = self.get_layout(cache.num_heads, -(-key[3] // self.block) * self.block)
+        elif layout.size(0) not in (1, cache.num_heads):
+            raise ValueError(f'a layout of {layout.size(0)} heads does not fit a cache of {cache.num_heads}')
+        meta = tables.build_meta(layout)
+        op = self._attn[key] = _lib.ops().CacheAttentionOp(meta.hdr, meta.on(device), self.block)
+        return op
 
 
 SparseSelfAttention = DeepSpeedSparseSelfAttention

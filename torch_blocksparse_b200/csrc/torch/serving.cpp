@@ -146,6 +146,96 @@ std::pair<Tensor, OptTensor> rotary_call(const c10::intrusive_ptr<RotaryOp>& p, 
   return {yq, yk.defined() ? OptTensor(yk) : OptTensor()};
 }
 
+// ---- the 4-bit cache ---------------------------------------------------------------------------
+struct CacheOp : torch::CustomClassHolder {
+  Tensor data;                             // [pages, heads, page bytes] uint8
+  int64_t page, head_dim;
+  int64_t pages() const { return data.size(0); }
+  int64_t heads() const { return data.size(1); }
+};
+
+// int32 [Z] on the cache's device, without gaps.
+const int32_t* per_sequence(const OptTensor& t, int64_t Z, const CacheOp& c, const char* what) {
+  if (!t) return nullptr;
+  TORCH_CHECK(t->device() == c.data.device(), what, " is on ", t->device(), ", the cache on ", c.data.device());
+  TORCH_CHECK_VALUE(t->scalar_type() == at::kInt && t->dim() == 1 && t->size(0) == Z && (Z < 2 || t->stride(0) == 1), what,
+                    " must be int32 [", Z, "] without gaps (got ", t->scalar_type(), " ", t->sizes(), ")");
+  return t->const_data_ptr<int32_t>();
+}
+struct PageTable {
+  const int32_t* at;
+  int64_t stride, slots;
+};
+PageTable page_table(const Tensor& t, int64_t Z, const CacheOp& c) {
+  TORCH_CHECK(t.device() == c.data.device(), "the page table is on ", t.device(), ", the cache on ", c.data.device());
+  TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == Z && (t.size(1) < 2 || t.stride(1) == 1),
+                    "pages must be int32 [", Z, ", slots] with unit stride on the slots (got ", t.scalar_type(), " ", t.sizes(), ")");
+  return {t.const_data_ptr<int32_t>(), t.stride(0), t.size(1)};
+}
+// Nothing in a cache is differentiable: an operand that wants a gradient would lose it silently.
+void no_gradient(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!recorded(t), what, " needs a gradient, which the cache does not give; call under torch.no_grad()");
+}
+Tensor unit_rows(const Tensor& x) { return x.stride(3) == 1 ? x : x.clone(at::MemoryFormat::Contiguous); }
+
+void cache_write(const c10::intrusive_ptr<CacheOp>& c, const Tensor& k0, const Tensor& v0, const Tensor& pages, const Tensor& start,
+                 const OptTensor& count) {
+  TORCH_CHECK_VALUE(k0.dim() == 4 && k0.size(1) == c->heads() && k0.size(3) == c->head_dim && v0.sizes() == k0.sizes(),
+                    "key and value must be [Z, ", c->heads(), ", T, ", c->head_dim, "] (got ", k0.sizes(), ", ", v0.sizes(), ")");
+  require_cuda(k0);
+  TORCH_CHECK(k0.device() == c->data.device(), "the key is on ", k0.device(), ", the cache on ", c->data.device());
+  require_same(v0, k0, "the value");
+  const int code = dtype_code(k0);
+  no_gradient(k0, "the key");
+  no_gradient(v0, "the value");
+  const c10::cuda::CUDAGuard guard(k0.device());
+  const Tensor k = unit_rows(k0), v = unit_rows(v0);
+  const int64_t Z = k.size(0);
+  const PageTable t = page_table(pages, Z, *c);
+  check(bsp_cache_write(k.const_data_ptr(), v.const_data_ptr(), code, Z, c->heads(), k.size(2), c->head_dim, k.stride(0), k.stride(1),
+                        k.stride(2), v.stride(0), v.stride(1), v.stride(2), c->data.mutable_data_ptr(), c->pages(), c->page, t.at,
+                        t.stride, t.slots, per_sequence(start, Z, *c, "start"), per_sequence(count, Z, *c, "count"), stream_of(k)));
+}
+
+std::pair<Tensor, Tensor> cache_read(const c10::intrusive_ptr<CacheOp>& c, const Tensor& pages, const Tensor& start, int64_t length,
+                                     const OptTensor& count, at::ScalarType type) {
+  TORCH_CHECK_VALUE(start.dim() == 1 && length >= 0 && length <= INT32_MAX, "cannot read ", length, " tokens from ", start.sizes());
+  const c10::cuda::CUDAGuard guard(c->data.device());
+  const int64_t Z = start.size(0);
+  const PageTable t = page_table(pages, Z, *c);
+  const auto options = c->data.options().dtype(type);
+  const Tensor k = at::empty({Z, c->heads(), length, c->head_dim}, options), v = at::empty(k.sizes(), options);
+  check(bsp_cache_read(k.mutable_data_ptr(), v.mutable_data_ptr(), dtype_code(k), Z, c->heads(), length, c->head_dim, k.stride(0), k.stride(1),
+                       k.stride(2), v.stride(0), v.stride(1), v.stride(2), c->data.const_data_ptr(), c->pages(), c->page, t.at, t.stride,
+                       t.slots, per_sequence(start, Z, *c, "start"), per_sequence(count, Z, *c, "count"), stream_of(k)));
+  return {k, v};
+}
+
+// ---- attention over the cache --------------------------------------------------------------------
+struct CacheAttentionOp : torch::CustomClassHolder {
+  Tensor hdr, meta;                        // header (host) and tables (device) of the layout
+  int64_t block;
+};
+
+Tensor cache_attention(const c10::intrusive_ptr<CacheAttentionOp>& p, const Tensor& q0, const c10::intrusive_ptr<CacheOp>& c,
+                       const Tensor& pages, const Tensor& lengths, double scale) {
+  TORCH_CHECK_VALUE(q0.dim() == 4 && q0.size(3) == c->head_dim && q0.size(1) % c->heads() == 0, "query must be [Z, n * ", c->heads(),
+                    ", T, ", c->head_dim, "] for this cache (got ", q0.sizes(), ")");
+  require_cuda(q0);
+  TORCH_CHECK(q0.device() == c->data.device(), "the query is on ", q0.device(), ", the cache on ", c->data.device());
+  const int code = dtype_code(q0);
+  no_gradient(q0, "the query");
+  const c10::cuda::CUDAGuard guard(q0.device());
+  const Tensor q = unit_rows(q0), o = at::empty(q.sizes(), q.options());
+  const int64_t Z = q.size(0);
+  const PageTable t = page_table(pages, Z, *c);
+  check(bsp_cache_attn(q.const_data_ptr(), o.mutable_data_ptr(), code, Z, q.size(1), c->heads(), q.size(2), c->head_dim, q.stride(0),
+                       q.stride(1), q.stride(2), o.stride(0), o.stride(1), o.stride(2), c->data.const_data_ptr(), c->pages(), c->page,
+                       t.at, t.stride, t.slots, per_sequence(lengths, Z, *c, "lengths"), p->block, p->hdr.const_data_ptr<int32_t>(),
+                       p->meta.const_data_ptr<int32_t>(), static_cast<float>(scale), stream_of(q)));
+  return o;
+}
+
 }  // namespace
 
 void bind_serving(pybind11::module_& m) {
@@ -159,4 +249,19 @@ void bind_serving(pybind11::module_& m) {
       .def("__call__", &rotary_call, py::call_guard<py::gil_scoped_release>())
       .def("one", [](const c10::intrusive_ptr<RotaryOp>& p, const Tensor& x, const OptTensor& pos) { return rotary_call(p, x, {}, pos).first; },
            py::call_guard<py::gil_scoped_release>());
+  py::class_<CacheOp, c10::intrusive_ptr<CacheOp>>(m, "CacheOp")
+      .def(py::init([](Tensor data, int64_t page, int64_t head_dim) {
+        auto c = c10::make_intrusive<CacheOp>();
+        c->data = data; c->page = page; c->head_dim = head_dim;
+        return c;
+      }))
+      .def("write", &cache_write, py::call_guard<py::gil_scoped_release>())
+      .def("read", &cache_read, py::call_guard<py::gil_scoped_release>());
+  py::class_<CacheAttentionOp, c10::intrusive_ptr<CacheAttentionOp>>(m, "CacheAttentionOp")
+      .def(py::init([](Tensor hdr, Tensor meta, int64_t block) {
+        auto p = c10::make_intrusive<CacheAttentionOp>();
+        p->hdr = hdr; p->meta = meta; p->block = block;
+        return p;
+      }))
+      .def("__call__", &cache_attention, py::call_guard<py::gil_scoped_release>());
 }
