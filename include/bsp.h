@@ -560,7 +560,7 @@ int bsp_cache_read(void* k, void* v, int dtype, int Z, int H, int T, int D,
  * sequence z stands at position lengths[z] - T + t (DEVICE [Z]) and sees the keys at
  * positions up to its own that lie in the nonzero blocks of its block-row:
  * o = softmax(scale * q K^T) V.  q, o [Z, Hq, T, D] (FP16 or BF16, unit stride
- * on D); query head h reads head h / (Hq / Hk) of the cache.  meta: metadata
+ * on D; q's other strides even, its base on 4 bytes); query head h reads head h / (Hq / Hk) of the cache.  meta: metadata
  * of a square layout of 1 or Hk heads.  Queries that see nothing (positions below
  * zero or behind the layout's last row, pages that are none) give zeros.
  */

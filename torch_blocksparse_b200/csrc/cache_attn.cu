@@ -26,11 +26,13 @@
 //
 // Work: a CTA's warps, times the CTAs of a cluster, take the granules of one (sequence, head, eight
 // queries) in turn, each through a ring of its own (cp.async, no barriers), and join their sums
-// once, in shared memory, then over the cluster in a fixed order: results do not depend on timing.
-#include <cooperative_groups.h>
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_runtime.h>
+// once, in shared memory, then by sending them over the cluster, in a fixed order: results do not depend on timing.
+//
+// What bounds it now: instructions.  A granule of 128 channels takes an SM's quarter 490 cycles; loading alone takes 375 (the
+// whole of the memory's rate).  Masks, shifts, packing and maxima hold the issue port two cycles each (64 + 16 + 8 + 8 of
+// them), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one.  More warps an SM (96 or 80
+// registers) change nothing.  592 heads x sequences of 8192 keys, G = 4: bf16 138 us, 77 % of the copy rate.
+#include <algorithm>
 
 #include "cache.cuh"
 #include "common.h"
@@ -41,12 +43,15 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kWarps = 8;
-constexpr int kStages = 4;
+constexpr int kWarps = 4;
+constexpr int kStages = 2;
+constexpr int kCtas = 4;            // on an SM
 constexpr int kQueries = 8;
-constexpr float kLowest = -3e38f;  // a maximum that nothing has entered
+constexpr int kMaxCluster = 8;
+constexpr float kNothing = -3e38f; // the maximum of no scores
 constexpr float kSlack = 4.f;      // p <= 2^4
-constexpr uint32_t kEights = 0x00080008u;
+constexpr uint32_t kEights = 0x00080008u;        // halves 8 * 2^-24
+constexpr int kNone = 0x7ffffff0;  // the token of a granule that is not there: nobody sees it
 
 struct AttnParams {
   const void* q;
@@ -62,247 +67,317 @@ struct AttnParams {
 };
 
 __device__ __forceinline__ void mma_half(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same on top of c0, c1 in both halves of the rows.
+__device__ __forceinline__ void mma_half_from(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1,
+                                              float c0, float c1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%10,%11};\n"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
   return y;
 }
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(to), "l"(from));
+}
 __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float exact_exp2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
-__device__ __forceinline__ float bf16_at(uint32_t pair, int i) { return __uint_as_float(i ? pair & 0xffff0000u : pair << 16); }
+__device__ __forceinline__ int exponent_of(float x) { return max(-100, min(100, static_cast<int>(__float_as_uint(x) >> 23) - 127)); }
+// One of a pair of bf16 as a float, and times another (exact: 16 significant bits).  Both on the FMA pipe in one instruction:
+// a shift or mask takes the integer pipe two cycles, and that pipe is what the kernel runs out of.
+__device__ __forceinline__ float bf16_at(uint32_t pair, int i) {
+  float x;
+  if (i) asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.bf16 %0, h, 0f00000000;}" : "=f"(x) : "r"(pair));
+  else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.bf16 %0, l, 0f00000000;}" : "=f"(x) : "r"(pair));
+  return x;
+}
+__device__ __forceinline__ float bf16_product(uint32_t pair, uint32_t other, int i) {
+  float x;
+  if (i) asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, h, n, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
+  else asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, l, m, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
+  return x;
+}
+__device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
 
-// One stretch of a layout's row: granules of its blocks up to the last position that may be seen.
-struct Segment {
-  int begin, granules, last;       // first entry in blk_col; granules of all its blocks; last visible token
-};
-
-template <typename T, int D, bool SPLIT>
-__global__ void __launch_bounds__(kWarps * 32, 2) cache_attn_kernel(const __grid_constant__ AttnParams p) {
-  constexpr int REC = record_bytes(D), HALF = REC / 2, NC = D / 64, NG = D / kGroup, NK = D / 16;
+template <typename T, int D, bool SPLIT, int NP>
+__global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int REC = record_bytes(D), HALF = REC / 2, STAGE = NP * REC, NC = D / 64, NG = D / kGroup, NK = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
-  __shared__ int stage_token[kWarps][kStages];
-  __shared__ float part_m[kWarps][kQueries], part_l[kWarps][kQueries], cta_m[kQueries], cta_l[kQueries];
+  __shared__ uint4 q_operand[NG][32];              // of both quarters of a group, by lane
+  __shared__ float2 q_start[NG][4];                // by pair of queries
+  __shared__ int2 listed[kWarps][32];              // granules looked up: record, first token + row (0, 1)
+  __shared__ float part_m[kWarps][kQueries], part_l[kWarps][kQueries];
+  __shared__ float inbox[kQueries * D + kMaxCluster], inbox_m[kMaxCluster][kQueries], inbox_l[kMaxCluster][kQueries];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
-  uint8_t* ring = smem + warp * (kStages * REC);
+  uint8_t* ring = smem + warp * (kStages * STAGE);
 
-  // ---- which queries, which rows of the layout
+  if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n");   // (this CTA runs: others may write here)
+
+  // ---- which queries
   const int rank = blockIdx.x % p.cluster;
   int w = blockIdx.x / p.cluster;
   const int tile = w % p.tiles;
   w /= p.tiles;
   const int hk = w % p.pages.heads, z = w / p.pages.heads;
-  const int64_t len = p.lengths[z];
+  const int32_t* row_ptr = p.row_ptr + static_cast<int64_t>(p.layout_heads > 1 ? hk : 0) * p.layout_rows;
+  const int len = max(p.lengths[z], 0);
   const int r0 = tile * kQueries, nq = min(kQueries, p.T * p.G - r0);
-  auto position = [&](int r) { return len - p.T + (r0 + r) / p.G; };     // of query r of the tile; negative: there is none
-  Segment seg[2];
-  const int64_t last_pos = position(nq - 1);
-  int64_t first_pos = position(0);
-  if (first_pos < 0) first_pos = 0;
-  const int block_log2 = p.block_shift + 4;
-#pragma unroll
-  for (int s = 0; s < 2; ++s) {
-    // the first query's row, and the last one's if that is another (8 queries span at most 8 positions, a block 16)
-    const int64_t row = (s ? last_pos : first_pos) >> block_log2;
-    seg[s] = {0, 0, -1};
-    if (last_pos < 0 || row >= p.layout_rows || (s && row == first_pos >> block_log2)) continue;
-    const int64_t at = static_cast<int64_t>(p.layout_heads > 1 ? hk : 0) * p.layout_rows + row;
-    seg[s].begin = p.row_ptr[at];
-    seg[s].granules = (p.row_ptr[at + 1] - seg[s].begin) << p.block_shift;
-    seg[s].last = static_cast<int>(min(last_pos, ((row + 1) << block_log2) - 1));
-  }
-  // last visible token of this lane's two queries in each segment (-1: none), and what all queries see
-  int limit[2][2], all_see[2] = {INT32_MAX, INT32_MAX};
-#pragma unroll
-  for (int r = 0; r < kQueries; ++r) {
-    const int64_t pos = r < nq ? position(r) : -1;
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      const int64_t row = (s ? last_pos : first_pos) >> block_log2;
-      const int lim = pos >= 0 && pos >> block_log2 == row ? static_cast<int>(pos) : -1;
-      if (r < nq) all_see[s] = min(all_see[s], lim);
-      if (r / 2 == t4) limit[s][r % 2] = lim;
-    }
-  }
-
-  // ---- q as operands: fp16 scaled by a power of two, and what the codes' offset adds up to
-  uint32_t qf[NK][2];
-  float start[NG][2], unscale[2];
+  // (two channels a load: see the entry point)
+  uint32_t qraw[NK][2];
   {
-    const bool there = g < nq;
-    const int r = r0 + g;
-    const T* q = static_cast<const T*>(p.q) + z * p.q_sz + (hk * p.G + r % p.G) * p.q_sh + (r / p.G) * p.q_st;
-    float x[NK][4], amax = 0.f;
+    const int r = r0 + min(g, nq - 1), t = p.T == 1 ? 0 : r / p.G;
+    const T* q = static_cast<const T*>(p.q) + z * p.q_sz + (hk * p.G + r - t * p.G) * p.q_sh + t * p.q_st + t4 * 2;
 #pragma unroll
     for (int n = 0; n < NK; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[n][i] = there ? static_cast<float>(q[n * 16 + t4 * 2 + i % 2 + i / 2 * 8]) : 0.f;
-        amax = fmaxf(amax, fabsf(x[n][i]));
-      }
-    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-    // |q| < 2^(e + 1); q * 2^(13 - e) < 2^14, and a sixteenth of it in the odd quarters
-    const int e = max(-100, min(100, static_cast<int>(__float_as_uint(amax) >> 23) - 127));
-    const float up = exact_exp2(13 - e);
-    float sum[NG] = {};
+      for (int i = 0; i < 2; ++i) qraw[n][i] = *reinterpret_cast<const uint32_t*>(q + n * 16 + i * 8);
+  }
+
+  // ---- which rows of the layout: the first query's and, if that is another, the last one's (8 queries span
+  // at most 8 positions, a block at least 16); of each its entries in blk_col, the granules of all its blocks, and the
+  // last token that any query sees.  limit: that token for this lane's two queries (-1: none); all_see: what
+  // every query sees (-1: nothing is sure).
+  const int block_log2 = p.block_shift + 4;
+  int begin[2] = {0, 0}, granules[2] = {0, 0}, last[2] = {-1, -1}, limit[2][2], all_see;
+  {
+    const int first_pos = len - p.T + (p.T == 1 ? 0 : r0 / p.G), last_pos = len - p.T + (p.T == 1 ? 0 : (r0 + nq - 1) / p.G);
+    const int row[2] = {max(first_pos, 0) >> block_log2, last_pos >> block_log2};
 #pragma unroll
-    for (int n = 0; n < NK; ++n) {
-      const float f = n % 2 ? up * 0.0625f : up;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const __half2 h = __floats2half2_rn(x[n][2 * i] * f, x[n][2 * i + 1] * f);
-        qf[n][i] = *reinterpret_cast<const uint32_t*>(&h);
-        sum[n / 2] += (__half2float(h.x) + __half2float(h.y)) * (n % 2 ? 16.f : 1.f);
-      }
+    for (int s = 0; s < 2; ++s) {
+      limit[s][0] = limit[s][1] = s ? -1 : last_pos;
+      if (last_pos < 0 || row[s] >= p.layout_rows || (s && row[1] == row[0])) continue;
+      begin[s] = row_ptr[row[s]];
+      granules[s] = (row_ptr[row[s] + 1] - begin[s]) << p.block_shift;
+      last[s] = static_cast<int>(min(static_cast<int64_t>(last_pos), (static_cast<int64_t>(row[s] + 1) << block_log2) - 1));
     }
-    const float down = p.scale_log2e * exact_exp2(e) * 2048.f;           // 2^24 * 2^(e - 13)
+    all_see = first_pos >= 0 && row[0] == row[1] ? first_pos : -1;
+    if (p.T > 1) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      unscale[i] = __shfl_sync(~0u, down, (2 * t4 + i) * 4);
+      for (int s = 0; s < 2; ++s) {
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        float s = sum[k];
-        s += __shfl_xor_sync(~0u, s, 1);
-        s += __shfl_xor_sync(~0u, s, 2);
-        start[k][i] = __shfl_sync(~0u, s, (2 * t4 + i) * 4) * -0x1p-21f;
+        for (int i = 0; i < 2; ++i) {
+          const int r = 2 * t4 + i, pos = r < nq ? len - p.T + (r0 + r) / p.G : -1;
+          limit[s][i] = pos >= 0 && pos >> block_log2 == row[s] ? pos : -1;
+        }
       }
     }
   }
 
-  // ---- the warp's granules: number wid + n * nw of both segments, one after the other
-  const int total = seg[0].granules + seg[1].granules, nw = kWarps * p.cluster, wid = rank * kWarps + warp;
+  // ---- the warp's granules: number wid + n * nw of both rows, one after the other
+  const int nw = kWarps * p.cluster, wid = rank * kWarps + warp, total = granules[0] + granules[1];
   const int mine = total > wid ? (total - wid + nw - 1) / nw : 0;
-  int n0 = 0;
-  uint32_t found = 0;              // of the 32 last looked up, those that are not loaded yet
-  int64_t my_at = 0;
-  int my_token = 0;
-  // Loads the next granule that has a page and a visible token into `stage`; token 16 k + segment, -1: no more.
-  auto fetch = [&](int stage) {
-    while (found == 0 && n0 < mine) {
-      const int n = n0 + lane;
-      my_at = -1;
-      if (n < mine) {
-        int i = wid + n * nw;
-        const int s = i >= seg[0].granules;
-        if (s) i -= seg[0].granules;
-        const int begin = s ? seg[1].begin : seg[0].begin, last = s ? seg[1].last : seg[0].last;
-        const int gran = (p.blk_col[begin + (i >> p.block_shift)] << p.block_shift) + (i & ((1 << p.block_shift) - 1));
-        my_token = gran * kGranule + s;
-        if (gran * kGranule <= last) my_at = p.pages.granule(z, hk, gran);
-      }
-      found = __ballot_sync(~0u, my_at >= 0);
-      n0 += 32;
-    }
-    int token = -1;
-    if (found) {
-      const int src = __ffs(found) - 1;
-      found &= found - 1;
-      const int64_t at = __shfl_sync(~0u, my_at, src);
-      token = __shfl_sync(~0u, my_token, src);
-      const uint8_t* from = p.data + at * REC;
+  int n0 = 0, at = 0, found = 0;   // looked up so far; of the last 32 those loaded, and those to be loaded
+  const uint8_t* data = p.data + lane * 16;
+  const uint32_t ring_at = smem_u32(ring) + lane * 16;
+  // Loads the next NP granules that have a page and a visible token into a stage; their tokens + rows, kNone: no more.
+  auto fetch = [&](int stage_offset, int (&tokens)[NP]) {
 #pragma unroll
-      for (int i = 0; i < (REC / 16 + 31) / 32; ++i)
-        if (i * 32 + lane < REC / 16) cp_async16(ring + stage * REC + (i * 32 + lane) * 16, from + (i * 32 + lane) * 16, true);
+    for (int u = 0; u < NP; ++u) {
+      tokens[u] = kNone;
+      while (at == found && n0 < mine) {
+        const int n = n0 + lane;
+        int record = -1, first = 0;
+        if (n < mine) {
+          int i = wid + n * nw;
+          const int s = i >= granules[0];
+          if (s) i -= granules[0];
+          const int gran = (p.blk_col[(s ? begin[1] : begin[0]) + (i >> p.block_shift)] << p.block_shift) + (i & ((1 << p.block_shift) - 1));
+          first = gran * kGranule + s;
+          if (gran * kGranule <= (s ? last[1] : last[0])) record = static_cast<int>(p.pages.granule(z, hk, gran));
+        }
+        const uint32_t has = __ballot_sync(~0u, record >= 0);
+        if (record >= 0) listed[warp][__popc(has & ((1u << lane) - 1))] = make_int2(record, first);
+        __syncwarp();
+        at = 0;
+        found = __popc(has);
+        n0 += 32;
+      }
+      if (at < found) {
+        const int2 next = listed[warp][at++];
+        tokens[u] = next.y;
+        const uint8_t* from = data + static_cast<uint64_t>(static_cast<uint32_t>(next.x)) * REC;
+        const uint32_t to = ring_at + stage_offset + u * REC;
+#pragma unroll
+        for (int i = 0; i < REC / 512; ++i) copy16(to + i * 512, from + i * 512);
+        if (lane < REC / 16 % 32) copy16(to + REC / 512 * 512, from + REC / 512 * 512);
+      }
     }
-    if (lane == 0) stage_token[warp][stage] = token;
     cp_async_commit();
   };
+  int tokens[NP], ahead[NP];
+  fetch(0, tokens);
+  fetch(STAGE, ahead);
+
+  // ---- q as operands: halves scaled by a power of two, and what the codes' offset adds up to; one group of 32
+  // channels a warp, kept in shared memory (registers are what limits the warps of an SM)
+  float unscale[2];
+  {
+    auto pair_at = [&](int n, int i) {
+      if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&qraw[n][i]));
+      else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&qraw[n][i]));
+    };
+    float amax = 0.f;
+#pragma unroll
+    for (int n = 0; n < NK; ++n)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(pair_at(n, i).x), fabsf(pair_at(n, i).y)));
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
+    // |q| < 2^(e + 1); q * 2^(13 - e) < 2^14, and a sixteenth of it in the odd quarters
+    const int e = exponent_of(amax);
+    const float sign = p.scale_log2e > 0.f ? 1.f : p.scale_log2e < 0.f ? -1.f : p.scale_log2e;   // (scores come out scaled by > 0)
+    const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 2048.f, 0x1p-100f);          // 2^24 * 2^(e - 13)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) unscale[i] = __shfl_sync(~0u, down, (2 * t4 + i) * 4);
+    const float up = exact_exp2(13 - e) * sign;
+#pragma unroll
+    for (int k = 0; k < NG; ++k) {
+      if (k % kWarps != warp) continue;
+      uint32_t h[4];
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 x = pair_at(2 * k + j / 2, j % 2);
+        const float f = j / 2 ? up * 0.0625f : up;
+        h[j] = pack_half(x.x * f, x.y * f);
+        const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h[j]));
+        sum += (r.x + r.y) * (j / 2 ? 16.f : 1.f);
+      }
+      sum += __shfl_xor_sync(~0u, sum, 1);
+      sum += __shfl_xor_sync(~0u, sum, 2);
+      q_operand[k][lane] = make_uint4(h[0], h[1], h[2], h[3]);
+      if (t4 == 0) reinterpret_cast<float*>(q_start[k])[g] = sum * -0x1p-21f;
+    }
+  }
+  __syncthreads();
 
   float acc[NK][4] = {}, eights[NG][4] = {};       // O^T: 16 channels each by the queries; sums of P times 8 * 2^-24
-  float m[2] = {kLowest, kLowest}, l[2] = {0.f, 0.f};
-  float boost[NG], ceiling[NG];                    // powers of two on P; scales that make a new one due
+  // largest score before `unscale`; that it is time for a new one; minus the largest, scaled; sums of weights
+  float m[2] = {-INFINITY, -INFINITY}, limit_m[2] = {-INFINITY, -INFINITY}, neg_m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
+  uint32_t boost[NG / 2];                          // powers of two on P, pairs of bf16
+  __nv_bfloat162 ceiling[NG / 2];                  // scales of V above which new ones are due
 #pragma unroll
-  for (int k = 0; k < NG; ++k) boost[k] = ceiling[k] = 0.f;
+  for (int k = 0; k < NG / 2; ++k) {
+    boost[k] = 0;
+    ceiling[k] = as_bf162(0);
+  }
 
-#pragma unroll
-  for (int s = 0; s < kStages - 1; ++s) fetch(s);
-  for (int it = 0;; ++it) {
-    cp_async_wait<kStages - 2>();
+  // NP granules at a time: what is done once for them (waiting, voting, branching) is a good part of the work,
+  // and they hide each other's latencies
+  for (int stage = 0;; stage ^= STAGE) {
+    cp_async_wait<kStages - 1>();
     __syncwarp();
-    const int mark = stage_token[warp][it % kStages];
-    if (mark < 0) break;
-    fetch((it + kStages - 1) % kStages);
-    const uint8_t* rec = ring + it % kStages * REC;
-    const int token = mark & ~15, s = mark & 15;
+    if (tokens[0] == kNone) break;
+    const uint8_t* rec = ring + stage;
 
-    // scores of tokens token + g and token + g + 8 for queries 2 t4 and 2 t4 + 1
-    uint32_t ks[2][NG / 2], vs[2][NG / 2];
+    // scores of tokens g and g + 8 for queries 2 t4 and 2 t4 + 1 (before `unscale`)
+    uint32_t ks[NP][2][NG / 2], vs[NP][2][NG / 2];
+    float x[NP][4];
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < NG / 2; ++k) {
-        ks[i][k] = reinterpret_cast<const uint32_t*>(rec + 8 * D)[(g + 8 * i) * (NG / 2) + k];
-        vs[i][k] = reinterpret_cast<const uint32_t*>(rec + HALF + 8 * D)[(g + 8 * i) * (NG / 2) + k];
-      }
-    float sc[4] = {};
-#pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      uint4 x = reinterpret_cast<const uint4*>(rec + c * 512)[lane];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int k = 2 * c + half, n = 4 * c + 2 * half;
-        float a[4] = {start[k][0], start[k][1], start[k][0], start[k][1]};
-        mma_half(a, x.x & 0x000f000fu, x.y & 0x000f000fu, x.z & 0x000f000fu, x.w & 0x000f000fu, qf[n][0], qf[n][1]);
-        mma_half(a, x.x & 0x00f000f0u, x.y & 0x00f000f0u, x.z & 0x00f000f0u, x.w & 0x00f000f0u, qf[n + 1][0], qf[n + 1][1]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = fmaf(a[i], bf16_at(ks[i / 2][k / 2], k % 2), sc[i]);
-        x.x >>= 8; x.y >>= 8; x.z >>= 8; x.w >>= 8;
-      }
-    }
-    float sv[2][NG];
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int k = 0; k < NG; ++k) sv[i][k] = bf16_at(vs[i][k / 2], k % 2);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) sc[i] *= unscale[i % 2];
-    bool see[4] = {true, true, true, true};
-    const bool masked = token + 15 > (s ? all_see[1] : all_see[0]);
-    if (masked) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        see[i] = token + g + 8 * (i / 2) <= (s ? limit[1][i % 2] : limit[0][i % 2]);
-        if (!see[i]) sc[i] = -INFINITY;
-      }
+    for (int u = 0; u < NP; ++u)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
-        if (!see[2 * i] && !see[2 * i + 1])
 #pragma unroll
-          for (int k = 0; k < NG; ++k) sv[i][k] = 0.f;
+        for (int k = 0; k < NG / 2; ++k) {
+          ks[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + 8 * D)[(g + 8 * i) * (NG / 2) + k];
+          vs[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + HALF + 8 * D)[(g + 8 * i) * (NG / 2) + k];
+        }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) {
+      uint4 w[NP];
+#pragma unroll
+      for (int u = 0; u < NP; ++u) w[u] = reinterpret_cast<const uint4*>(rec + u * REC + c * 512)[lane];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int k = 2 * c + half;
+        const uint4 qf = q_operand[k][lane];
+        const float2 start = q_start[k][t4];
+#pragma unroll
+        for (int u = 0; u < NP; ++u) {
+          float a[4];
+          mma_half_from(a, w[u].x & 0x000f000fu, w[u].y & 0x000f000fu, w[u].z & 0x000f000fu, w[u].w & 0x000f000fu, qf.x, qf.y, start.x, start.y);
+          mma_half(a, w[u].x & 0x00f000f0u, w[u].y & 0x00f000f0u, w[u].z & 0x00f000f0u, w[u].w & 0x00f000f0u, qf.z, qf.w);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float s = bf16_at(ks[u][i / 2][k / 2], k % 2);
+            x[u][i] = k ? fmaf(a[i], s, x[u][i]) : a[i] * s;
+          }
+          w[u].x >>= 8; w[u].y >>= 8; w[u].z >>= 8; w[u].w >>= 8;
+        }
+      }
+    }
+    // take out what some queries do not see
+    uint32_t keep[NP][2];                          // halves of P that their query sees
+    const bool masked = tokens[NP - 1] + 15 > all_see;   // (a row's tokens ascend; where there are two rows, all_see is -1)
+    if (masked) {
+#pragma unroll
+      for (int u = 0; u < NP; ++u) {
+        const int token = (tokens[u] & ~15) + g;
+        const bool s = tokens[u] & 15;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const bool a = token + 8 * i <= (s ? limit[1][0] : limit[0][0]), b = token + 8 * i <= (s ? limit[1][1] : limit[0][1]);
+          keep[u][i] = (a ? 0x0000ffffu : 0u) | (b ? 0xffff0000u : 0u);
+          if (!a) x[u][2 * i] = -INFINITY;
+          if (!b) x[u][2 * i + 1] = -INFINITY;
+          if (!a && !b)
+#pragma unroll
+            for (int k = 0; k < NG / 2; ++k) vs[u][i][k] = 0;
+        }
+      }
     }
 
-    bool due = fmaxf(sc[0], sc[2]) > m[0] + kSlack || fmaxf(sc[1], sc[3]) > m[1] + kSlack;
+    // renew the maxima and powers of two where they are exceeded
+    float top[2];
+    __nv_bfloat162 scale_top[NG / 2];
 #pragma unroll
-    for (int k = 0; k < NG; ++k) due = due || fmaxf(sv[0][k], sv[1][k]) > ceiling[k];
-    if (__any_sync(~0u, due)) {
+    for (int u = 0; u < NP; ++u) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) top[i] = u ? fmaxf(top[i], fmaxf(x[u][i], x[u][i + 2])) : fmaxf(x[u][i], x[u][i + 2]);
+#pragma unroll
+      for (int k = 0; k < NG / 2; ++k) {
+        const __nv_bfloat162 s = __hmax2(as_bf162(vs[u][0][k]), as_bf162(vs[u][1][k]));
+        scale_top[k] = u ? __hmax2(scale_top[k], s) : s;
+      }
+    }
+    uint32_t over = 0;
+#pragma unroll
+    for (int k = 0; k < NG / 2; ++k) over |= __hgt2_mask(scale_top[k], ceiling[k]);
+    if (__any_sync(~0u, top[0] > limit_m[0] || top[1] > limit_m[1] || over)) {
       float f[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        float x = fmaxf(sc[i], sc[i + 2]);
+        float t = top[i];
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
-        x = fmaxf(x, m[i]);
-        f[i] = fast_exp2(m[i] - x);
-        m[i] = x;
+        for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+        f[i] = 1.f;
+        if (t > m[i]) {
+          f[i] = fast_exp2((m[i] - t) * unscale[i]);
+          m[i] = t;
+          neg_m[i] = -t * unscale[i];
+          limit_m[i] = t + kSlack / unscale[i];
+        }
         l[i] *= f[i];
       }
 #pragma unroll
       for (int k = 0; k < NG; ++k) {
-        float x = fmaxf(sv[0][k], sv[1][k]), ratio = 1.f;
+        float t = k % 2 ? __high2float(scale_top[k / 2]) : __low2float(scale_top[k / 2]), ratio = 1.f;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) x = fmaxf(x, __shfl_xor_sync(~0u, x, d));
-        if (x > ceiling[k]) {                      // the largest scale becomes 2^7 .. 2^8 in P
-          const int e = max(-100, min(100, static_cast<int>(__float_as_uint(x) >> 23) - 127));
-          const float b = exact_exp2(7 - e);
-          ratio = boost[k] > 0.f ? b / boost[k] : 0.f;
-          boost[k] = b;
-          ceiling[k] = exact_exp2(e + 4);
+        for (int d = 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+        if (t > (k % 2 ? __high2float(ceiling[k / 2]) : __low2float(ceiling[k / 2]))) {
+          const int e = exponent_of(t);            // the largest scale becomes 2^7 .. 2^8 in P
+          const float b = exact_exp2(7 - e), old = bf16_at(boost[k / 2], k % 2);
+          ratio = old > 0.f ? b / old : 0.f;
+          boost[k / 2] = k % 2 ? (boost[k / 2] & 0xffffu) | __float_as_uint(b) : (boost[k / 2] & 0xffff0000u) | __float_as_uint(b) >> 16;
+          const __nv_bfloat16 c = __float2bfloat16_rn(exact_exp2(e + 4));
+          ceiling[k / 2] = k % 2 ? __halves2bfloat162(__low2bfloat16(ceiling[k / 2]), c) : __halves2bfloat162(c, __high2bfloat16(ceiling[k / 2]));
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -313,129 +388,138 @@ __global__ void __launch_bounds__(kWarps * 32, 2) cache_attn_kernel(const __grid
       }
     }
 
-    float pr[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      pr[i] = fast_exp2(sc[i] - m[i % 2]);
-      l[i % 2] += pr[i];
-    }
+    for (int u = 0; u < NP; ++u)
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-      uint4 x = reinterpret_cast<const uint4*>(rec + HALF + c * 512)[lane];
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        const int k = 2 * c + half, n = 4 * c + 2 * half;
-        float pw[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          pw[i] = pr[i] * (sv[i / 2][k] * boost[k]);
-          if (masked && !see[i]) pw[i] = 0.f;      // (a NaN scale of a token that this query does not see)
-        }
-        const uint32_t h0 = pack_half(pw[0], pw[1]), h1 = pack_half(pw[2], pw[3]);
-        const uint32_t b0 = transpose8(h0), b1 = transpose8(h1);
-        const uint4 lo = make_uint4(x.x & 0x000f000fu, x.y & 0x000f000fu, x.z & 0x000f000fu, x.w & 0x000f000fu);
-        const uint4 hi = make_uint4(x.x & 0x00f000f0u, x.y & 0x00f000f0u, x.z & 0x00f000f0u, x.w & 0x00f000f0u);
-        mma_half(acc[n], lo.x, lo.y, lo.z, lo.w, b0, b1);
-        mma_half(acc[n + 1], hi.x, hi.y, hi.z, hi.w, b0, b1);
-        mma_half(eights[k], kEights, kEights, kEights, kEights, b0, b1);
-        if constexpr (SPLIT) {
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-          const uint32_t c0 = transpose8(pack_half(pw[0] - f0.x, pw[1] - f0.y)), c1 = transpose8(pack_half(pw[2] - f1.x, pw[3] - f1.y));
-          mma_half(acc[n], lo.x, lo.y, lo.z, lo.w, c0, c1);
-          mma_half(acc[n + 1], hi.x, hi.y, hi.z, hi.w, c0, c1);
-          mma_half(eights[k], kEights, kEights, kEights, kEights, c0, c1);
-        }
-        x.x >>= 8; x.y >>= 8; x.z >>= 8; x.w >>= 8;
+      for (int i = 0; i < 4; ++i) {
+        x[u][i] = fast_exp2(fmaf(x[u][i], unscale[i % 2], neg_m[i % 2]));
+        l[i % 2] += x[u][i];
       }
-    }
+    auto add_values = [&](auto some_unseen) {
+#pragma unroll
+      for (int u = 0; u < NP; ++u)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+          uint4 w = reinterpret_cast<const uint4*>(rec + u * REC + HALF + c * 512)[lane];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int k = 2 * c + half, n = 4 * c + 2 * half;
+            const float s0 = bf16_product(vs[u][0][k / 2], boost[k / 2], k % 2), s1 = bf16_product(vs[u][1][k / 2], boost[k / 2], k % 2);
+            uint32_t h0 = pack_half(x[u][0] * s0, x[u][1] * s0), h1 = pack_half(x[u][2] * s1, x[u][3] * s1);
+            if constexpr (some_unseen) {           // (0 times a NaN scale of a token that this query does not see)
+              h0 &= keep[u][0];
+              h1 &= keep[u][1];
+            }
+            const uint4 lo = make_uint4(w.x & 0x000f000fu, w.y & 0x000f000fu, w.z & 0x000f000fu, w.w & 0x000f000fu);
+            const uint4 hi = make_uint4(w.x & 0x00f000f0u, w.y & 0x00f000f0u, w.z & 0x00f000f0u, w.w & 0x00f000f0u);
+            auto add = [&](uint32_t p0, uint32_t p1) {
+              const uint32_t b0 = transpose8(p0), b1 = transpose8(p1);
+              mma_half(acc[n], lo.x, lo.y, lo.z, lo.w, b0, b1);
+              mma_half(acc[n + 1], hi.x, hi.y, hi.z, hi.w, b0, b1);
+              mma_half(eights[k], kEights, kEights, kEights, kEights, b0, b1);
+            };
+            add(h0, h1);
+            if constexpr (SPLIT) {
+              const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
+              h0 = pack_half(x[u][0] * s0 - f0.x, x[u][1] * s0 - f0.y);
+              h1 = pack_half(x[u][2] * s1 - f1.x, x[u][3] * s1 - f1.y);
+              if constexpr (some_unseen) {
+                h0 &= keep[u][0];
+                h1 &= keep[u][1];
+              }
+              add(h0, h1);
+            }
+            w.x >>= 8; w.y >>= 8; w.z >>= 8; w.w >>= 8;
+          }
+        }
+    };
+    if (masked) add_values(std::true_type());
+    else add_values(std::false_type());
+    __syncwarp();                                  // (all lanes are done with the stage)
+#pragma unroll
+    for (int u = 0; u < NP; ++u) tokens[u] = ahead[u];
+    fetch(stage, ahead);
   }
   cp_async_wait<0>();
   __syncwarp();
 
   // ---- join: the warp's sums into its ring, then all warps', then all CTAs' of the cluster
-  float* mine_o = reinterpret_cast<float*>(ring);  // [8 queries][D]
+  float* own = reinterpret_cast<float*>(ring);     // [queries][D]
 #pragma unroll
   for (int k = 0; k < NG; ++k) {
-    const float back = boost[k] > 0.f ? 1.f / boost[k] : 0.f;
+    const float b = bf16_at(boost[k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
 #pragma unroll
-    for (int half = 0; half < 2; ++half)
+    for (int i = 0; i < 2; ++i)
+      if (2 * t4 + i < nq)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float v = (acc[2 * k + half][i] * (half ? 0.0625f : 1.f) - eights[k][i]) * 0x1p24f * back;
-        mine_o[(2 * t4 + i % 2) * D + (2 * k + half) * 16 + g + i / 2 * 8] = v;
-      }
+        for (int j = 0; j < 4; ++j)                // channel g + 8 j of the group
+          own[(2 * t4 + i) * D + k * 32 + g + 8 * j] =
+              (acc[2 * k + j / 2][i + j % 2 * 2] * (j / 2 ? 0.0625f : 1.f) - eights[k][i]) * 0x1p24f * back;
   }
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) l[i] += __shfl_xor_sync(~0u, l[i], d);
     if (g == 0) {
-      part_m[warp][2 * t4 + i] = m[i];
+      part_m[warp][2 * t4 + i] = l[i] > 0.f || l[i] != l[i] ? -neg_m[i] : kNothing;
       part_l[warp][2 * t4 + i] = l[i];
     }
   }
   __syncthreads();
-  const bool alone = p.cluster == 1;
   T* o = static_cast<T*>(p.o) + z * p.o_sz;
-  auto store = [&](int r, int d, float v) {
-    const int q = r0 + r;
-    o[(hk * p.G + q % p.G) * p.o_sh + (q / p.G) * p.o_st + d] = cvt_out<T>(v);
+  auto store = [&](int r, int d, float sum, float weight) {
+    const int q = r0 + r, t = p.T == 1 ? 0 : q / p.G;
+    o[(hk * p.G + q - t * p.G) * p.o_sh + t * p.o_st + d] = cvt_out<T>(weight > 0.f || weight != weight ? sum / weight : 0.f);
   };
-  float* joined = reinterpret_cast<float*>(smem);
-  constexpr int PER = kQueries * D / (kWarps * 32);
-  float sums[PER];
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int at = i * kWarps * 32 + threadIdx.x, r = at / D;
-    if (r >= nq) break;
-    float top = kLowest, sum = 0.f, weight = 0.f;
+  // Where there are more CTAs, each sends every one of them the part of the sums that it stores in the end: rank v
+  // has v * share .. v * share + share - 1.
+  const int share = (nq * D + p.cluster - 1) / p.cluster;
+  cg::cluster_group cluster = cg::this_cluster();
+  if (p.cluster > 1) asm volatile("barrier.cluster.wait.aligned;\n");
+  for (int at = threadIdx.x; at < nq * D; at += kWarps * 32) {
+    const int r = at / D;
+    float top = kNothing, sum = 0.f, weight = 0.f;
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) top = fmaxf(top, part_m[v][r]);
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) {
       const float f = fast_exp2(part_m[v][r] - top);
       weight += part_l[v][r] * f;
-      sum += reinterpret_cast<const float*>(smem + v * (kStages * REC))[at] * f;
+      sum += reinterpret_cast<const float*>(smem + v * (kStages * STAGE))[at] * f;
     }
-    if (alone) {
-      store(r, at % D, weight > 0.f || weight != weight ? sum / weight : 0.f);
-    } else {
-      sums[i] = sum;
-      if (at % D == 0) {
-        cta_m[r] = top;
-        cta_l[r] = weight;
-      }
+    if (p.cluster == 1) {
+      store(r, at % D, sum, weight);
+      continue;
+    }
+    const int to = at / share;
+    cluster.map_shared_rank(inbox, to)[rank * share + at - to * share] = sum;
+    if (at % D < p.cluster) {
+      cluster.map_shared_rank(&inbox_m[rank][r], at % D)[0] = top;
+      cluster.map_shared_rank(&inbox_l[rank][r], at % D)[0] = weight;
     }
   }
-  if (alone) return;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < PER; ++i) {
-    const int at = i * kWarps * 32 + threadIdx.x;
-    if (at / D >= nq) break;
-    joined[at] = sums[i];
-  }
-  cg::cluster_group cluster = cg::this_cluster();
+  if (p.cluster == 1) return;
   cluster.sync();
-  const int share = (nq * D + p.cluster - 1) / p.cluster;
-  for (int at = rank * share + threadIdx.x; at < min((rank + 1) * share, nq * D); at += kWarps * 32) {
-    const int r = at / D;
-    float top = kLowest, sum = 0.f, weight = 0.f;
-    for (int v = 0; v < p.cluster; ++v) top = fmaxf(top, *cluster.map_shared_rank(&cta_m[r], v));
-    for (int v = 0; v < p.cluster; ++v) {
-      const float f = fast_exp2(*cluster.map_shared_rank(&cta_m[r], v) - top);
-      weight += *cluster.map_shared_rank(&cta_l[r], v) * f;
-      sum += *cluster.map_shared_rank(&joined[at], v) * f;
-    }
-    store(r, at % D, weight > 0.f || weight != weight ? sum / weight : 0.f);
+  for (int i = threadIdx.x; i < share && rank * share + i < nq * D; i += kWarps * 32) {
+    const int at = rank * share + i, r = at / D;
+    float top = kNothing, sum = 0.f, weight = 0.f;
+#pragma unroll
+    for (int v = 0; v < kMaxCluster; ++v)
+      if (v < p.cluster) top = fmaxf(top, inbox_m[v][r]);
+#pragma unroll
+    for (int v = 0; v < kMaxCluster; ++v)
+      if (v < p.cluster) {
+        const float f = fast_exp2(inbox_m[v][r] - top);
+        weight += inbox_l[v][r] * f;
+        sum += inbox[v * share + i] * f;
+      }
+    store(r, at % D, sum, weight);
   }
-  cluster.sync();                  // (nobody's shared memory goes before all have read it)
 }
 
-template <typename T, int D> int launch(const AttnParams& p, int64_t groups, cudaStream_t stream) {
-  constexpr bool split = sizeof(T) == 2 && std::is_same_v<T, __half>;
-  constexpr int bytes = kWarps * kStages * record_bytes(D);
-  auto kernel = cache_attn_kernel<T, D, split>;
+template <typename T, int D, int NP> int launch(const AttnParams& p, int64_t groups, cudaStream_t stream) {
+  constexpr int bytes = kWarps * kStages * NP * record_bytes(D);
+  auto kernel = cache_attn_kernel<T, D, std::is_same_v<T, __half>, NP>;
   static thread_local bool ready[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
@@ -485,6 +569,12 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   if (Z == 0 || T == 0 || Hq == 0) return BSP_OK;
   if (!q || !o || !lengths || (slots && !pages) || (num_pages && !data)) return fail(BSP_ERR_INVALID, "cache attention: NULL argument");
   if (reinterpret_cast<uintptr_t>(data) & 15) return fail(BSP_ERR_INVALID, "cache attention: the cache is not 16-byte aligned");
+  if ((static_cast<int64_t>(num_pages) * Hk) << log2_of(page / kGranule) > INT32_MAX) return fail(BSP_ERR_UNSUPPORTED, "cache attention: caches of up to 2^31 times 16 tokens");
+  uint64_t odd = reinterpret_cast<uintptr_t>(q) >> 1;    // queries are read two channels at a time
+  if (Z > 1) odd |= q_sz;
+  if (Hq > 1) odd |= q_sh;
+  if (T > 1) odd |= q_st;
+  if ((odd & 1) || (reinterpret_cast<uintptr_t>(q) & 1)) return fail(BSP_ERR_INVALID, "cache attention: queries need even strides and a base on 4 bytes");
   const Meta mt = meta_view(meta, meta_hdr[1], meta_hdr[2], meta_hdr[3], meta_hdr[4], meta_hdr[5], meta_hdr[6]);
   AttnParams p;
   p.q = q; p.o = o;
@@ -499,12 +589,19 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   p.tiles = (T * p.G + kQueries - 1) / kQueries;
   p.scale_log2e = scale * 1.4426950408889634f;
   const int64_t groups = static_cast<int64_t>(Z) * Hk * p.tiles;
-  // CTAs of a cluster: enough to fill two on every SM, no more than give every warp four granules of the longest row
-  const int64_t granules = static_cast<int64_t>(mt.max_row) << p.block_shift;
-  p.cluster = 1;
-  while (p.cluster < 8 && groups * p.cluster < 2 * 148 && granules > 4 * kWarps * p.cluster) p.cluster *= 2;
+  // CTAs of a cluster: as many as fit the SMs at once (one sequence of 12 heads, 36 blocks of 64: 8 CTAs 5.4 us, one 6.4;
+  // 8 x 16 heads: 4 CTAs 10.7 us, 8 CTAs, which do not fit, 16.5), and a granule of an average row for every warp.
+  // Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys: 107 us, one at a
+  // time 111); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 12.4 us, one at a time 10.7).
+  const int64_t granules = (static_cast<int64_t>(mt.nnz) / (static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
+  p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * 148 / groups, granules / kWarps})));
+  const bool many = granules > 16 * kWarps * p.cluster;
   if (Z > INT32_MAX / Hk / p.tiles / p.cluster) return fail(BSP_ERR_UNSUPPORTED, "cache attention: too many queries");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == BSP_F16) return D == 64 ? launch<__half, 64>(p, groups, s) : launch<__half, 128>(p, groups, s);
-  return D == 64 ? launch<__nv_bfloat16, 64>(p, groups, s) : launch<__nv_bfloat16, 128>(p, groups, s);
+  if (many) {
+    if (dtype == BSP_F16) return D == 64 ? launch<__half, 64, 4>(p, groups, s) : launch<__half, 128, 2>(p, groups, s);
+    return D == 64 ? launch<__nv_bfloat16, 64, 4>(p, groups, s) : launch<__nv_bfloat16, 128, 2>(p, groups, s);
+  }
+  if (dtype == BSP_F16) return D == 64 ? launch<__half, 64, 1>(p, groups, s) : launch<__half, 128, 1>(p, groups, s);
+  return D == 64 ? launch<__nv_bfloat16, 64, 1>(p, groups, s) : launch<__nv_bfloat16, 128, 1>(p, groups, s);
 }

@@ -44,8 +44,8 @@ Positions positions_of(const OptTensor& pos, const RotaryOp& p, const Tensor& q)
   return r;
 }
 
-// Rows with a unit stride; neighbouring pairs also on a boundary of a pair's size.
-Tensor rotary_rows(const Tensor& x, bool pairs) {
+// Rows with a unit stride; where they are read in pairs, also on a boundary of a pair's size.
+Tensor even_rows(const Tensor& x, bool pairs) {
   const int64_t even = pairs ? 2 : 1;
   bool ok = x.stride(3) == 1 && reinterpret_cast<uintptr_t>(x.const_data_ptr()) % (even * x.element_size()) == 0;
   for (int i = 0; i < 3; ++i) ok = ok && (x.size(i) == 1 || x.stride(i) % even == 0);
@@ -66,7 +66,7 @@ std::pair<Tensor, Tensor> rotary(const RotaryOp& p, const OptTensor& q0, const O
   for (int i = 0; i < 2; ++i) {
     const OptTensor& t = i ? k0 : q0;
     if (!t) continue;
-    x[i] = rotary_rows(*t, p.interleaved);
+    x[i] = even_rows(*t, p.interleaved);
     y[i] = rotary_out(x[i]);
     for (int j = 0; j < 3; ++j) {
       s[i][j] = x[i].stride(j);
@@ -226,7 +226,7 @@ Tensor cache_attention(const c10::intrusive_ptr<CacheAttentionOp>& p, const Tens
   const int code = dtype_code(q0);
   no_gradient(q0, "the query");
   const c10::cuda::CUDAGuard guard(q0.device());
-  const Tensor q = unit_rows(q0), o = at::empty(q.sizes(), q.options());
+  const Tensor q = even_rows(q0, true), o = at::empty(q.sizes(), q.options());
   const int64_t Z = q.size(0);
   const PageTable t = page_table(pages, Z, *c);
   check(bsp_cache_attn(q.const_data_ptr(), o.mutable_data_ptr(), code, Z, q.size(1), c->heads(), q.size(2), c->head_dim, q.stride(0),
