@@ -32,6 +32,10 @@
 // whole of the memory's rate).  Masks, shifts, packing and maxima hold the issue port two cycles each (64 + 16 + 8 + 8 of
 // them), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one.  More warps an SM (96 or 80
 // registers) change nothing.  592 heads x sequences of 8192 keys, G = 4: bf16 138 us, 77 % of the copy rate.
+#include <cooperative_groups.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
 #include <algorithm>
 
 #include "cache.cuh"
