@@ -48,44 +48,55 @@ template <typename T, bool VEC> __device__ __forceinline__ uint4 load8(const T* 
   }
 }
 
+__device__ __forceinline__ float2 to_f2(__half2 v) { return __half22float2(v); }
+__device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622float2(v); }
+
 // The codes + 8 of 8 channels, two in each word (bits 0-3 and 16-19), and the scale of their group, which 4
 // neighbouring lanes hold together.
 //
-// rint(x / s) without a division, and equal to it: with |x / s| < 8, r = 1/s rounded to nearest and x of at
+// rint(x / s) without a division, and equal to it: with |x / s| < 8, r within 2^-23 of 1 / s and x of at
 // most 11 significant bits, s of 8, a quotient that is no tie is at least 2^-13 away from one, x * r at most
 // 2^-20 away from the quotient.  So x * r rounded to a multiple of 2^-16 (an FMA that adds 192, where
 // floats are 2^-16 apart) lies on the same side of a tie, or on the tie itself if the quotient
-// is one, and adding 1.5 * 2^23 + 8 then rounds it to an even integer that ends in c + 8.
+// is one, and taking 192 off and adding 1.5 * 2^23 + 8 in one sum then rounds it to an even integer that ends in c + 8.
+// max / 7 is the rounded product with 1 / 7 and one step of correction by its exact remainder, which gives the
+// rounded quotient (checked over both types' values, with the rest, by the tests).
 template <typename T> __device__ __forceinline__ uint32_t quantise8(uint4 raw, uint32_t (&pair)[4]) {
   using T2 = typename Two<T>::t;
   const uint32_t in[4] = {raw.x, raw.y, raw.z, raw.w};
   T2 v[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = *reinterpret_cast<const T2*>(&in[i]);
-  const T2 m2 = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])), __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
-  T m = __hmax_nan(m2.x, m2.y);
-  m = __hmax_nan(m, __shfl_xor_sync(~0u, m, 2));    // (lanes sub ^ 1, sub ^ 2 share the group)
-  m = __hmax_nan(m, __shfl_xor_sync(~0u, m, 1));
-  const float amax = static_cast<float>(m);
-  __nv_bfloat16 sb = __float2bfloat16_rn(__fdiv_rn(amax, 7.f));
-  if (!(amax < INFINITY)) sb = __ushort_as_bfloat16(0x7fff);
-  const float s = __bfloat162float(sb);
-  if (s > 1e-30f) {
-    const float r = __frcp_rn(s);
+  T2 m2 = __hmax2_nan(__hmax2_nan(__habs2(v[0]), __habs2(v[1])), __hmax2_nan(__habs2(v[2]), __habs2(v[3])));
+  m2 = __hmax2_nan(m2, __shfl_xor_sync(~0u, m2, 2));    // (lanes sub ^ 1, sub ^ 2 share the group)
+  m2 = __hmax2_nan(m2, __shfl_xor_sync(~0u, m2, 1));
+  const float amax = static_cast<float>(__hmax_nan(m2.x, m2.y));
+  constexpr float kSeventh = 1.f / 7.f;
+  const float q0 = amax * kSeventh;
+  const __nv_bfloat16 fast = __float2bfloat16_rn(__fmaf_rn(__fmaf_rn(-7.f, q0, amax), kSeventh, q0));
+  if (amax > 1e-29f && amax < INFINITY) {
+    const float s = __bfloat162float(fast);
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(s));
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const float a = (__fmaf_rn(static_cast<float>(v[i].x), r, 192.f) - 192.f) + (12582912.f + 8.f);
-      const float b = (__fmaf_rn(static_cast<float>(v[i].y), r, 192.f) - 192.f) + (12582912.f + 8.f);
+      const float2 x = to_f2(v[i]);
+      const float a = __fadd_rn(__fmaf_rn(x.x, r, 192.f), 12582912.f + 8.f - 192.f);
+      const float b = __fadd_rn(__fmaf_rn(x.y, r, 192.f), 12582912.f + 8.f - 192.f);
       pair[i] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x5410) & 0x000f000fu;
     }
-  } else {                                          // zeros, NaN, or scales whose reciprocal a float does not hold
+    return __bfloat16_as_ushort(fast);
+  }
+  // zeros, infinities, NaN, or scales whose reciprocal a float does not hold
+  const __nv_bfloat16 sb = amax < INFINITY ? __float2bfloat16_rn(__fdiv_rn(amax, 7.f)) : __ushort_as_bfloat16(0x7fff);
+  const float s = __bfloat162float(sb);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      float c[2] = {static_cast<float>(v[i].x), static_cast<float>(v[i].y)};
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = to_f2(v[i]);
+    float c[2] = {x.x, x.y};
 #pragma unroll
-      for (int j = 0; j < 2; ++j) c[j] = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(c[j], s)), -8.f), 7.f) : 0.f;
-      pair[i] = static_cast<uint32_t>(static_cast<int>(c[0]) + 8) | static_cast<uint32_t>(static_cast<int>(c[1]) + 8) << 16;
-    }
+    for (int j = 0; j < 2; ++j) c[j] = s > 0.f ? fminf(fmaxf(rintf(__fdiv_rn(c[j], s)), -8.f), 7.f) : 0.f;
+    pair[i] = static_cast<uint32_t>(static_cast<int>(c[0]) + 8) | static_cast<uint32_t>(static_cast<int>(c[1]) + 8) << 16;
   }
   return __bfloat16_as_ushort(sb);
 }
@@ -101,9 +112,27 @@ __device__ __forceinline__ uint32_t gather_fields(const uint32_t (&pair)[4], int
   return (odd ? k1 : k0) | __shfl_xor_sync(~0u, odd ? k0 : k1, 2);
 }
 
+// What a lane of a token writes, by the token's place j in the granule: for every K or V one word (of K) or two half words (of V),
+// and for one lane of each group the scale.
+template <int D> struct Places {
+  int sub, c, n, h;
+  __device__ __forceinline__ explicit Places(int lane) : sub(lane % (D / 8)), c(sub / 8), n(sub / 2 % 4), h(sub % 2) {}
+  __device__ __forceinline__ void put(uint8_t* granule, int kv, int j, uint32_t word, uint32_t scale) const {
+    uint8_t* codes = granule + kv * (record_bytes(D) / 2);
+    if (kv == 0) {                                  // word n: channels 16 n' + 8 h + 2 n, + 1 of all quarters n'
+      *reinterpret_cast<uint32_t*>(codes + word_at(c, j % 8, n, j / 8 + 2 * h)) = word;
+    } else {                                        // half words: channels 8 h + 2 n and 8 h + 2 n + 1
+      uint8_t* q = codes + word_at(c, 2 * n, j % 8 / 2, h + 2 * (j / 8)) + 2 * (j % 2);
+      *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(word);
+      *reinterpret_cast<uint16_t*>(q + 64) = static_cast<uint16_t>(word >> 16);
+    }
+    if (sub % 4 == 0) *reinterpret_cast<uint16_t*>(codes + 8 * D + j * (2 * D / kGroup) + sub / 4 * 2) = static_cast<uint16_t>(scale);
+  }
+};
+
 template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) cache_write_kernel(const __grid_constant__ WriteParams p) {
-  constexpr int LPT = D / 8, TPI = 32 / LPT, ITER = kGranule / TPI, REC = record_bytes(D), HALF = REC / 2;
+  constexpr int REC = record_bytes(D);
   __shared__ __align__(16) uint8_t image[kWarps][REC];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int64_t id = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
@@ -117,41 +146,57 @@ __global__ void __launch_bounds__(kWarps * 32) cache_write_kernel(const __grid_c
   if (t0 >= count) return;
   const int64_t at = p.pages.granule(z, head, g);   // (negative positions have none)
   if (at < 0) return;
-  const bool whole = t0 >= 0 && t0 + kGranule <= count;
   uint8_t* record = p.data + at * REC;
-  uint8_t* dst = whole ? image[warp] : record;
-  const int sub = lane % LPT, c = sub / 8, n = sub / 2 % 4, h = sub % 2;
+  constexpr int LPT = D / 8, TPI = 32 / LPT, ITER = kGranule / TPI;
+  const Places<D> to(lane);
+  const int own = lane / LPT;
+  const T* x[2];
 #pragma unroll
-  for (int kv = 0; kv < 2; ++kv) {
-    const T* x = static_cast<const T*>(p.x[kv]) + z * p.sz[kv] + head * p.sh[kv] + sub * 8;
-    uint4 raw[ITER];
+  for (int kv = 0; kv < 2; ++kv)
+    x[kv] = static_cast<const T*>(p.x[kv]) + z * p.sz[kv] + head * p.sh[kv] + (t0 + own) * p.st[kv] + to.sub * 8;
+  if (t0 >= 0 && t0 + kGranule <= count) {
+    // all 16 tokens: put together in shared memory and stored 16 bytes at a time
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      const int64_t t = t0 + it * TPI + lane / LPT;
-      raw[it] = t >= 0 && t < count ? load8<T, VEC>(x + t * p.st[kv]) : make_uint4(0, 0, 0, 0);
-    }
-    uint8_t* codes = dst + kv * HALF;
+    for (int kv = 0; kv < 2; ++kv) {
+      uint4 raw[ITER];
 #pragma unroll
-    for (int it = 0; it < ITER; ++it) {
-      const int j = it * TPI + lane / LPT;
-      uint32_t pair[4];
-      const uint32_t scale = quantise8<T>(raw[it], pair);
-      const uint32_t word = gather_fields(pair, n);
-      if (t0 + j < 0 || t0 + j >= count) continue;
-      if (kv == 0) {                                // word n: channels 16 n' + 8 h + 2 n, + 1 of all quarters n'
-        *reinterpret_cast<uint32_t*>(codes + word_at(c, j % 8, n, j / 8 + 2 * h)) = word;
-      } else {                                      // half words: channels 8 h + 2 n and 8 h + 2 n + 1
-        uint8_t* q = codes + word_at(c, 2 * n, j % 8 / 2, h + 2 * (j / 8)) + 2 * (j % 2);
-        *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(word);
-        *reinterpret_cast<uint16_t*>(q + 64) = static_cast<uint16_t>(word >> 16);
+      for (int it = 0; it < ITER; ++it) raw[it] = load8<T, VEC>(x[kv] + it * TPI * p.st[kv]);
+      // (of a token's place only what depends on the lane is computed: steps of 8 / TPI go through places 0 .. 7)
+      uint8_t* base = image[warp];
+#pragma unroll
+      for (int it = 0; it < ITER; ++it) {
+        uint32_t pair[4];
+        const uint32_t scale = quantise8<T>(raw[it], pair);
+        const uint32_t word = gather_fields(pair, to.n);
+        const int j = it * TPI;
+        if (kv == 0) *reinterpret_cast<uint32_t*>(base + word_at(to.c, own, to.n, 2 * to.h) + word_at(0, j % 8, 0, j / 8)) = word;
+        else {
+          uint8_t* q = base + REC / 2 + word_at(to.c, 2 * to.n, own / 2, to.h) + 2 * (own % 2) + word_at(0, 0, j % 8 / 2, 2 * (j / 8));
+          *reinterpret_cast<uint16_t*>(q) = static_cast<uint16_t>(word);
+          *reinterpret_cast<uint16_t*>(q + 64) = static_cast<uint16_t>(word >> 16);
+        }
+        if (to.sub % 4 == 0)
+          *reinterpret_cast<uint16_t*>(base + kv * (REC / 2) + 8 * D + own * (2 * D / kGroup) + to.sub / 4 * 2 + j * (2 * D / kGroup)) = static_cast<uint16_t>(scale);
       }
-      if (sub % 4 == 0) *reinterpret_cast<uint16_t*>(codes + 8 * D + (j * (D / kGroup) + sub / 4) * 2) = static_cast<uint16_t>(scale);
     }
-  }
-  if (whole) {
     __syncwarp();
-    for (int i = lane; i < REC / 16; i += 32)
-      reinterpret_cast<uint4*>(record)[i] = reinterpret_cast<const uint4*>(image[warp])[i];
+#pragma unroll
+    for (int i = 0; i < (REC / 16 + 31) / 32; ++i)
+      if (i * 32 + lane < REC / 16) reinterpret_cast<uint4*>(record)[i * 32 + lane] = reinterpret_cast<const uint4*>(image[warp])[i * 32 + lane];
+  } else {
+    // some of them (a single new token, most of the time): in the pieces that belong to one token
+    const int end = static_cast<int>(min(count - t0, static_cast<int64_t>(kGranule)));
+    for (int j = t0 < 0 ? static_cast<int>(-t0) : 0; j < end; j += TPI) {
+      const bool there = j + own < end;
+      const uint4 k = there ? load8<T, VEC>(x[0] + j * p.st[0]) : make_uint4(0, 0, 0, 0);
+      const uint4 v = there ? load8<T, VEC>(x[1] + j * p.st[1]) : make_uint4(0, 0, 0, 0);
+      uint32_t pair[4];
+      uint32_t scale = quantise8<T>(k, pair), word = gather_fields(pair, to.n);
+      if (there) to.put(record, 0, j + own, word, scale);
+      scale = quantise8<T>(v, pair);
+      word = gather_fields(pair, to.n);
+      if (there) to.put(record, 1, j + own, word, scale);
+    }
   }
 }
 

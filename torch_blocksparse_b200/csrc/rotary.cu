@@ -26,7 +26,6 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTokens = 8;      // tokens of a CTA
-constexpr int kBatch = 2;          // rows that a thread has under way at a time
 
 struct RotaryTensor {
   const void* x;
@@ -50,28 +49,60 @@ template <typename T> __device__ __forceinline__ float to_f(T v) { return static
 
 template <typename T, int VEC> struct alignas(sizeof(T) * VEC) Vec { T v[VEC]; };
 
+// (through uint4: the compiler splits accesses of the struct itself, 51 -> 59 us for 8192 tokens x 2 x 32 heads of 128)
+template <typename V> __device__ __forceinline__ V load_v(const void* p) {
+  if constexpr (sizeof(V) == 16) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p);
+    return *reinterpret_cast<const V*>(&x);
+  } else {
+    return *reinterpret_cast<const V*>(p);
+  }
+}
+template <typename V> __device__ __forceinline__ void store_v(void* p, const V& v) {
+  if constexpr (sizeof(V) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&v);
+  else *reinterpret_cast<V*>(p) = v;
+}
+
 // A unit is VEC elements of the first half and their partners in the second (!INTER), VEC neighbouring
 // elements (INTER), or VEC elements behind the turned ones.
 template <typename T, int VEC, bool INTER>
-__global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant__ RotaryParams p) {
+__global__ void __launch_bounds__(kThreads, VEC == 8 && !INTER ? 5 : 4) rotary_kernel(const __grid_constant__ RotaryParams p) {
+  // Heads that a thread has under way at a time: with the sines of 8 pairs in registers, more warps do more than a second one
+  // (8192 tokens x 2 x 32 heads of 128: one 51 us, two 58, four 75; with fewer sines the other way round: FP32, 3219 tokens x 15 heads of 80, 9.5 and 8.9 us).
+  constexpr int kBatch = VEC == 8 && !INTER ? 1 : 2;
   extern __shared__ float2 cs[];                    // [tokens][pairs]
-  __shared__ int tz[kMaxTokens], tl[kMaxTokens];
   const int tid = threadIdx.x, tokens = 1 << p.log_tokens;
   const int64_t first = static_cast<int64_t>(blockIdx.x) << p.log_tokens, total = static_cast<int64_t>(p.Z) * p.L;
-  if (tid < tokens) {
-    const int64_t n = first + tid;
-    tz[tid] = n < total ? static_cast<int>(n / p.L) : -1;
-    tl[tid] = static_cast<int>(n % p.L);
-  }
-  __syncthreads();
+  // A thread keeps one unit of one token, and so its sines, for every head that it takes.
+  const int u = tid & ((1 << p.log_units) - 1), tok = tid >> p.log_units & (tokens - 1);
+  const int h0 = tid >> (p.log_units + p.log_tokens), step = kThreads >> (p.log_units + p.log_tokens);
+  const int turned = INTER ? 2 * p.pairs / VEC : p.pairs / VEC, rest = (p.D - 2 * p.pairs) / VEC;
+  const bool works = u < turned + rest && first + tok < total, tail = u >= turned;
+  const int d = tail ? 2 * p.pairs + (u - turned) * VEC : u * VEC, far = INTER || tail ? 0 : p.pairs;
+  const int64_t z = (first + tok) / p.L, l = (first + tok) - z * p.L;
+  using V = Vec<T, VEC>;
+  V a[kBatch], b[kBatch];
+  auto load = [&](int h) {
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      int head = h + i * step;
+      if (!works || head >= p.heads) continue;
+      const RotaryTensor& t = p.t[head >= p.heads0];
+      if (head >= p.heads0) head -= p.heads0;
+      const T* x = static_cast<const T*>(t.x) + z * t.x_sz + l * t.x_sl + head * t.x_sh + d;
+      a[i] = load_v<V>(x);
+      if (far) b[i] = load_v<V>(x + far);
+    }
+  };
+
   for (int i = tid; i < p.pairs << p.log_tokens; i += kThreads) {
-    const int tok = i / p.pairs, pr = i - tok * p.pairs, z = tz[tok], l = tl[tok];
-    if (z < 0) continue;
-    const int64_t a = p.table[p.pairs + pr];
-    const int64_t axis = a < 0 ? 0 : a < p.axes ? a : p.axes - 1;
-    int64_t pos = l;
+    const int n = i / p.pairs, pr = i - n * p.pairs;
+    if (first + n >= total) break;
+    const int64_t zn = (first + n) / p.L, ln = (first + n) - zn * p.L;
+    const int64_t axis = max(static_cast<int64_t>(0), min(p.table[p.pairs + pr], static_cast<int64_t>(p.axes - 1)));
+    int64_t pos = ln;
     if (p.pos_bytes) {
-      const int64_t at = axis * p.p_sa + z * p.p_sz + l * p.p_sl;
+      const int64_t at = axis * p.p_sa + zn * p.p_sz + ln * p.p_sl;
       pos = p.pos_bytes == 4 ? static_cast<const int32_t*>(p.positions)[at] : static_cast<const int64_t*>(p.positions)[at];
     }
     const int64_t turn = static_cast<int64_t>(static_cast<uint64_t>(pos) * static_cast<uint64_t>(p.table[pr]));
@@ -80,59 +111,40 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const __grid_constant_
     cs[i] = make_float2(c, p.inverse ? -s : s);
   }
   __syncthreads();
+  if (!works) return;
+  constexpr int NCS = INTER ? (VEC + 1) / 2 : VEC;
+  float2 w[NCS];
+#pragma unroll
+  for (int j = 0; j < NCS; ++j) w[j] = tail ? make_float2(1.f, 0.f) : cs[tok * p.pairs + (INTER ? d / 2 : d) + j];
 
-  const int units = 1 << p.log_units, u = tid & (units - 1), step = kThreads >> p.log_units;
-  const int turned = INTER ? 2 * p.pairs / VEC : p.pairs / VEC, rest = (p.D - 2 * p.pairs) / VEC;
-  if (u >= turned + rest) return;
-  const int rows = p.heads << p.log_tokens;
-  using V = Vec<T, VEC>;
-  const bool tail = u >= turned;
-  const int d = tail ? 2 * p.pairs + (u - turned) * VEC : u * VEC, far = INTER || tail ? 0 : p.pairs;
-  // kBatch rows at a time: their loads are under way together
-  for (int r0 = tid >> p.log_units; r0 < rows; r0 += kBatch * step) {
-    V a[kBatch], b[kBatch];
-    T* y[kBatch];
-    int tok[kBatch];
+  for (int h = h0; h < p.heads; h += kBatch * step) {
+    load(h);
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int r = r0 + i * step;
-      tok[i] = r & (tokens - 1);
-      y[i] = nullptr;
-      if (r >= rows || tz[tok[i]] < 0) continue;
-      const int64_t z = tz[tok[i]], l = tl[tok[i]];
-      int h = r >> p.log_tokens;
-      const RotaryTensor& t = p.t[h >= p.heads0];
-      if (h >= p.heads0) h -= p.heads0;
-      const T* x = static_cast<const T*>(t.x) + z * t.x_sz + h * t.x_sh + l * t.x_sl + d;
-      y[i] = static_cast<T*>(t.y) + z * t.y_sz + h * t.y_sh + l * t.y_sl + d;
-      a[i] = *reinterpret_cast<const V*>(x);
-      if (far) b[i] = *reinterpret_cast<const V*>(x + far);
-    }
-#pragma unroll
-    for (int i = 0; i < kBatch; ++i) {
-      if (!y[i]) continue;
-      const float2* w = cs + tok[i] * p.pairs;
+      int head = h + i * step;
+      if (head >= p.heads) break;
+      const RotaryTensor& t = p.t[head >= p.heads0];
+      if (head >= p.heads0) head -= p.heads0;
       if (!tail) {
         if constexpr (INTER) {
 #pragma unroll
           for (int j = 0; j < VEC / 2; ++j) {
-            const float2 f = w[d / 2 + j];
             const float x0 = to_f(a[i].v[2 * j]), x1 = to_f(a[i].v[2 * j + 1]);
-            a[i].v[2 * j] = cvt_out<T>(x0 * f.x - x1 * f.y);
-            a[i].v[2 * j + 1] = cvt_out<T>(x1 * f.x + x0 * f.y);
+            a[i].v[2 * j] = cvt_out<T>(x0 * w[j].x - x1 * w[j].y);
+            a[i].v[2 * j + 1] = cvt_out<T>(x1 * w[j].x + x0 * w[j].y);
           }
         } else {
 #pragma unroll
           for (int j = 0; j < VEC; ++j) {
-            const float2 f = w[d + j];
             const float x0 = to_f(a[i].v[j]), x1 = to_f(b[i].v[j]);
-            a[i].v[j] = cvt_out<T>(x0 * f.x - x1 * f.y);
-            b[i].v[j] = cvt_out<T>(x1 * f.x + x0 * f.y);
+            a[i].v[j] = cvt_out<T>(x0 * w[j].x - x1 * w[j].y);
+            b[i].v[j] = cvt_out<T>(x1 * w[j].x + x0 * w[j].y);
           }
         }
       }
-      *reinterpret_cast<V*>(y[i]) = a[i];
-      if (far) *reinterpret_cast<V*>(y[i] + far) = b[i];
+      T* y = static_cast<T*>(t.y) + z * t.y_sz + l * t.y_sl + head * t.y_sh + d;
+      store_v(y, a[i]);
+      if (far) store_v(y + far, b[i]);
     }
   }
 }
@@ -142,7 +154,7 @@ template <typename T, int VEC, bool INTER> int launch(RotaryParams& p, cudaStrea
   for (p.log_units = 0; (1 << p.log_units) < units; ++p.log_units) {}
   const int64_t total = static_cast<int64_t>(p.Z) * p.L;
   // more tokens a CTA while every SM still gets several
-  for (p.log_tokens = 0; (2 << p.log_tokens) <= kMaxTokens && total >> p.log_tokens >= 2048; ++p.log_tokens) {}
+  for (p.log_tokens = 0; (2 << p.log_tokens) <= kMaxTokens && total >> p.log_tokens >= 2048 && p.log_units + p.log_tokens < 8; ++p.log_tokens) {}
   const int64_t grid = (total + (1 << p.log_tokens) - 1) >> p.log_tokens;
   if (grid > INT32_MAX) return fail(BSP_ERR_UNSUPPORTED, "rotary: too many tokens (%lld)", (long long)total);
   rotary_kernel<T, VEC, INTER><<<static_cast<unsigned>(grid), kThreads, sizeof(float2) * p.pairs << p.log_tokens, stream>>>(p);
