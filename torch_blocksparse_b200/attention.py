@@ -221,14 +221,14 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         One kernel, without workspace, on the current stream of the cache's device; no gradient.  Lengths
         and tables are read on the device, so that a captured call can be replayed as sequences grow."""
         cache_op = cache._op()
-        key = ('decode', query.get_device(), cache.num_heads, None if self.layout is not None else pages.size(-1) * cache.page)
+        key = (cache_op.heads, query.get_device(), None if self.layout is not None else pages.size(-1) * cache.page, 'decode')
         op = self._attn.get(key) or self._decode_op(key, cache, query.device)
-        return op(query, cache_op, pages, lengths, float(query.size(-1)) ** -0.5 if scale is None else float(scale))
+        return op(query, cache_op, pages, lengths, scale)
 
     def _decode_op(self, key, cache, device):
         layout = self.layout
         if layout is None:
-            layout = self.get_layout(cache.num_heads, -(-key[3] // self.block) * self.block)
+            layout = self.get_layout(cache.num_heads, -(-key[2] // self.block) * self.block)
         elif layout.size(0) not in (1, cache.num_heads):
             raise ValueError(f'a layout of {layout.size(0)} heads does not fit a cache of {cache.num_heads}')
         meta = tables.build_meta(layout)

@@ -1,5 +1,6 @@
 // Host path of rotary positions, the 4-bit key / value cache and attention over it.
 #include <ATen/ops/empty_like.h>
+#include <cmath>
 
 #include "host.h"
 
@@ -218,7 +219,7 @@ struct CacheAttentionOp : torch::CustomClassHolder {
 };
 
 Tensor cache_attention(const c10::intrusive_ptr<CacheAttentionOp>& p, const Tensor& q0, const c10::intrusive_ptr<CacheOp>& c,
-                       const Tensor& pages, const Tensor& lengths, double scale) {
+                       const Tensor& pages, const Tensor& lengths, std::optional<double> scale) {
   TORCH_CHECK_VALUE(q0.dim() == 4 && q0.size(3) == c->head_dim && q0.size(1) % c->heads() == 0, "query must be [Z, n * ", c->heads(),
                     ", T, ", c->head_dim, "] for this cache (got ", q0.sizes(), ")");
   require_cuda(q0);
@@ -232,7 +233,7 @@ Tensor cache_attention(const c10::intrusive_ptr<CacheAttentionOp>& p, const Tens
   check(bsp_cache_attn(q.const_data_ptr(), o.mutable_data_ptr(), code, Z, q.size(1), c->heads(), q.size(2), c->head_dim, q.stride(0),
                        q.stride(1), q.stride(2), o.stride(0), o.stride(1), o.stride(2), c->data.const_data_ptr(), c->pages(), c->page,
                        t.at, t.stride, t.slots, per_sequence(lengths, Z, *c, "lengths"), p->block, p->hdr.const_data_ptr<int32_t>(),
-                       p->meta.const_data_ptr<int32_t>(), static_cast<float>(scale), stream_of(q)));
+                       p->meta.const_data_ptr<int32_t>(), static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(c->head_dim))), stream_of(q)));
   return o;
 }
 
@@ -255,6 +256,7 @@ void bind_serving(pybind11::module_& m) {
         c->data = data; c->page = page; c->head_dim = head_dim;
         return c;
       }))
+      .def_property_readonly("heads", &CacheOp::heads)
       .def("write", &cache_write, py::call_guard<py::gil_scoped_release>())
       .def("read", &cache_read, py::call_guard<py::gil_scoped_release>());
   py::class_<CacheAttentionOp, c10::intrusive_ptr<CacheAttentionOp>>(m, "CacheAttentionOp")
