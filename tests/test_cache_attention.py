@@ -123,6 +123,45 @@ def test_long_rows_are_split_over_a_cluster(dtype, Z, H, L, kind, block):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('G,T', [(1, 1), (1, 2), (2, 2), (4, 1), (8, 1)])
+def test_many_sequences_with_long_rows(dtype, D, G, T):
+    """As many heads as fill the GPU, each with more granules than a warp takes in sixteen steps; a few of them are checked."""
+    Z, H, L, block = 300, 2, 1203, 64
+    lengths = (L - torch.arange(Z) * 7 % 400).int().cuda()
+    layout = layouts.dense(1, -(-L // block))
+    layout[0, :, 3] = 0
+    slots = -(-L // 64)
+    cache, pages = Guarded(Z * slots, H, D), table(Z, slots, Z * slots)
+    k, v = tokens(Z, H, L, D, dtype), tokens(Z, H, L, D, dtype, 1)
+    zero = torch.zeros(Z, dtype=torch.int32, device='cuda')
+    cache.write(k, v, pages, zero, lengths)
+    del k, v
+    q = queries(Z, H * G, T, D, dtype)
+    got = SparseSelfAttention(layout=layout, block=block).decode(q, cache, pages, lengths)
+    some = torch.tensor([0, 1, 57, 58, 123, 299], device='cuda')
+    kk, vv = cache.read(pages[some], zero[some], L, lengths[some], dtype=torch.float32)
+    assert_decoded(got[some], q[some], kk, vv, torch.ones(6, L, dtype=torch.bool), lengths[some], layout, block, D ** -0.5)
+    alone = SparseSelfAttention(layout=layout, block=block).decode(q[some], cache, pages[some], lengths[some])
+    assert_decoded(alone, q[some], kk, vv, torch.ones(6, L, dtype=torch.bool), lengths[some], layout, block, D ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('H', [1, 74, 84, 98, 118, 148, 197, 296, 400])
+def test_every_size_of_cluster(H):
+    """The number of heads decides how many blocks of threads share a row: 8, 8, 7, 6, 5, 4, 3, 2 and 1 of them."""
+    L, D, block = 700, 64, 32
+    lengths = ints(L)
+    cache, pages, k, v = filled(1, H, L, D, 64, torch.float16, lengths)
+    layout = layouts.dense(1, -(-L // block))
+    q = queries(1, H, 3, D, torch.float16)
+    got = SparseSelfAttention(layout=layout, block=block).decode(q, cache, pages, lengths)
+    some = list(range(0, H, max(1, H // 9)))
+    assert_decoded(got[:, some], q[:, some], k[:, some], v[:, some], torch.ones(1, L, dtype=torch.bool), lengths, layout, block, D ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
 def test_scales_and_scores_that_grow_along_the_row(dtype):
     """Later keys outweigh earlier ones by far, and later values are larger (and the other way round)."""
     Z, L, D = 2, 700, 128

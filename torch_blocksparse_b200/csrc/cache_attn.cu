@@ -110,9 +110,12 @@ __device__ __forceinline__ float bf16_product(uint32_t pair, uint32_t other, int
 }
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
 
-template <typename T, int D, bool SPLIT, int NP>
+template <typename T, int D, bool SPLIT, bool FEW, int NP>
 __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __grid_constant__ AttnParams p) {
   constexpr int REC = record_bytes(D), HALF = REC / 2, STAGE = NP * REC, NC = D / 64, NG = D / kGroup, NK = D / 16;
+  // What a lane deals with: queries, and for each token pairs of groups of channels.  Two queries and all groups; with FEW, where
+  // queries x groups fit into 8, the columns of the products are (query, group) and a lane has one query and two groups.
+  constexpr int PAIRS = NG / 2, QL = FEW ? 1 : 2, SW = FEW ? 1 : PAIRS;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint4 q_operand[NG][32];              // of both quarters of a group, by lane
   __shared__ float2 q_start[NG][4];                // by pair of queries
@@ -121,6 +124,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   __shared__ float inbox[kQueries * D + kMaxCluster], inbox_m[kMaxCluster][kQueries], inbox_l[kMaxCluster][kQueries];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   uint8_t* ring = smem + warp * (kStages * STAGE);
+  const int my_query = FEW ? t4 / PAIRS : 2 * t4, my_pair = FEW ? t4 % PAIRS : 0;   // the first of them
+  const int q_column = FEW ? g / NG : g;           // the query of column g of the products
 
   if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n");   // (this CTA runs: others may write here)
 
@@ -136,7 +141,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   // (two channels a load: see the entry point)
   uint32_t qraw[NK][2];
   {
-    const int r = r0 + min(g, nq - 1), t = p.T == 1 ? 0 : r / p.G;
+    const int r = r0 + min(q_column, nq - 1), t = p.T == 1 ? 0 : r / p.G;
     const T* q = static_cast<const T*>(p.q) + z * p.q_sz + (hk * p.G + r - t * p.G) * p.q_sh + t * p.q_st + t4 * 2;
 #pragma unroll
     for (int n = 0; n < NK; ++n)
@@ -146,16 +151,17 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 
   // ---- which rows of the layout: the first query's and, if that is another, the last one's (8 queries span
   // at most 8 positions, a block at least 16); of each its entries in blk_col, the granules of all its blocks, and the
-  // last token that any query sees.  limit: that token for this lane's two queries (-1: none); all_see: what
+  // last token that any query sees.  limit: that token for this lane's queries (-1: none); all_see: what
   // every query sees (-1: nothing is sure).
   const int block_log2 = p.block_shift + 4;
-  int begin[2] = {0, 0}, granules[2] = {0, 0}, last[2] = {-1, -1}, limit[2][2], all_see;
+  int begin[2] = {0, 0}, granules[2] = {0, 0}, last[2] = {-1, -1}, limit[2][QL], all_see;
   {
     const int first_pos = len - p.T + (p.T == 1 ? 0 : r0 / p.G), last_pos = len - p.T + (p.T == 1 ? 0 : (r0 + nq - 1) / p.G);
     const int row[2] = {max(first_pos, 0) >> block_log2, last_pos >> block_log2};
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      limit[s][0] = limit[s][1] = s ? -1 : last_pos;
+#pragma unroll
+      for (int i = 0; i < QL; ++i) limit[s][i] = s ? -1 : last_pos;
       if (last_pos < 0 || row[s] >= p.layout_rows || (s && row[1] == row[0])) continue;
       begin[s] = row_ptr[row[s]];
       granules[s] = (row_ptr[row[s] + 1] - begin[s]) << p.block_shift;
@@ -166,8 +172,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = 2 * t4 + i, pos = r < nq ? len - p.T + (r0 + r) / p.G : -1;
+        for (int i = 0; i < QL; ++i) {
+          const int r = my_query + i, pos = r < nq ? len - p.T + (r0 + r) / p.G : -1;
           limit[s][i] = pos >= 0 && pos >> block_log2 == row[s] ? pos : -1;
         }
       }
@@ -221,7 +227,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 
   // ---- q as operands: halves scaled by a power of two, and what the codes' offset adds up to; one group of 32
   // channels a warp, kept in shared memory (registers are what limits the warps of an SM)
-  float unscale[2];
+  float unscale[QL], start[2];
   {
     auto pair_at = [&](int n, int i) {
       if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&qraw[n][i]));
@@ -239,7 +245,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     const float sign = p.scale_log2e > 0.f ? 1.f : p.scale_log2e < 0.f ? -1.f : p.scale_log2e;   // (scores come out scaled by > 0)
     const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 2048.f, 0x1p-100f);          // 2^24 * 2^(e - 13)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) unscale[i] = __shfl_sync(~0u, down, (2 * t4 + i) * 4);
+    for (int i = 0; i < QL; ++i) unscale[i] = __shfl_sync(~0u, down, (FEW ? my_query * NG : my_query + i) * 4);
     const float up = exact_exp2(13 - e) * sign;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
@@ -256,19 +262,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       }
       sum += __shfl_xor_sync(~0u, sum, 1);
       sum += __shfl_xor_sync(~0u, sum, 2);
-      q_operand[k][lane] = make_uint4(h[0], h[1], h[2], h[3]);
-      if (t4 == 0) reinterpret_cast<float*>(q_start[k])[g] = sum * -0x1p-21f;
+      const bool mine = !FEW || g % NG == k;       // (a column of another group: zeros)
+      q_operand[k][lane] = mine ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(0, 0, 0, 0);
+      if (t4 == 0 && mine) reinterpret_cast<float*>(q_start[FEW ? 0 : k])[g] = sum * -0x1p-21f;
     }
   }
   __syncthreads();
+  if constexpr (FEW) {
+    start[0] = q_start[0][t4].x;
+    start[1] = q_start[0][t4].y;
+  }
 
-  float acc[NK][4] = {}, eights[NG][4] = {};       // O^T: 16 channels each by the queries; sums of P times 8 * 2^-24
+  // O^T: 16 channels each by the columns (FEW: those of their own group count); sums of P times 8 * 2^-24
+  constexpr int NE = FEW ? 1 : NG;
+  float acc[NK][4] = {}, eights[NE][4] = {};
   // largest score before `unscale`; that it is time for a new one; minus the largest, scaled; sums of weights
-  float m[2] = {-INFINITY, -INFINITY}, limit_m[2] = {-INFINITY, -INFINITY}, neg_m[2] = {0.f, 0.f}, l[2] = {0.f, 0.f};
-  uint32_t boost[NG / 2];                          // powers of two on P, pairs of bf16
-  __nv_bfloat162 ceiling[NG / 2];                  // scales of V above which new ones are due
+  float m[QL], limit_m[QL], neg_m[QL], l[QL];
 #pragma unroll
-  for (int k = 0; k < NG / 2; ++k) {
+  for (int i = 0; i < QL; ++i) {
+    m[i] = limit_m[i] = -INFINITY;
+    neg_m[i] = l[i] = 0.f;
+  }
+  uint32_t boost[SW];                              // powers of two on P, pairs of bf16
+  __nv_bfloat162 ceiling[SW];                      // scales of V above which new ones are due
+#pragma unroll
+  for (int k = 0; k < SW; ++k) {
     boost[k] = 0;
     ceiling[k] = as_bf162(0);
   }
@@ -281,18 +299,19 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     if (tokens[0] == kNone) break;
     const uint8_t* rec = ring + stage;
 
-    // scores of tokens g and g + 8 for queries 2 t4 and 2 t4 + 1 (before `unscale`)
-    uint32_t ks[NP][2][NG / 2], vs[NP][2][NG / 2];
-    float x[NP][4];
+    // scores of tokens g (the first QL) and g + 8 for the lane's queries, before `unscale`
+    uint32_t ks[NP][2][SW], vs[NP][2][SW];
+    float x[NP][2 * QL];
 #pragma unroll
     for (int u = 0; u < NP; ++u)
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int k = 0; k < NG / 2; ++k) {
-          ks[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + 8 * D)[(g + 8 * i) * (NG / 2) + k];
-          vs[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + HALF + 8 * D)[(g + 8 * i) * (NG / 2) + k];
+        for (int k = 0; k < SW; ++k) {
+          ks[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + 8 * D)[(g + 8 * i) * PAIRS + my_pair + k];
+          vs[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + HALF + 8 * D)[(g + 8 * i) * PAIRS + my_pair + k];
         }
+    float sums[NP][2][4];                          // FEW: even and odd quarters, by (query, group)
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       uint4 w[NP];
@@ -302,20 +321,45 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       for (int half = 0; half < 2; ++half) {
         const int k = 2 * c + half;
         const uint4 qf = q_operand[k][lane];
-        const float2 start = q_start[k][t4];
+        if constexpr (!FEW) {
+          start[0] = q_start[k][t4].x;
+          start[1] = q_start[k][t4].y;
+        }
 #pragma unroll
         for (int u = 0; u < NP; ++u) {
-          float a[4];
-          mma_half_from(a, w[u].x & 0x000f000fu, w[u].y & 0x000f000fu, w[u].z & 0x000f000fu, w[u].w & 0x000f000fu, qf.x, qf.y, start.x, start.y);
-          mma_half(a, w[u].x & 0x00f000f0u, w[u].y & 0x00f000f0u, w[u].z & 0x00f000f0u, w[u].w & 0x00f000f0u, qf.z, qf.w);
+          const uint4 lo = make_uint4(w[u].x & 0x000f000fu, w[u].y & 0x000f000fu, w[u].z & 0x000f000fu, w[u].w & 0x000f000fu);
+          const uint4 hi = make_uint4(w[u].x & 0x00f000f0u, w[u].y & 0x00f000f0u, w[u].z & 0x00f000f0u, w[u].w & 0x00f000f0u);
+          if constexpr (FEW) {
+            if (k == 0) {
+              mma_half_from(sums[u][0], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y, start[0], start[1]);
+              mma_half_from(sums[u][1], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w, 0.f, 0.f);
+            } else {
+              mma_half(sums[u][0], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y);
+              mma_half(sums[u][1], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w);
+            }
+          } else {
+            float a[4];
+            mma_half_from(a, lo.x, lo.y, lo.z, lo.w, qf.x, qf.y, start[0], start[1]);
+            mma_half(a, hi.x, hi.y, hi.z, hi.w, qf.z, qf.w);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float s = bf16_at(ks[u][i / 2][k / 2], k % 2);
-            x[u][i] = k ? fmaf(a[i], s, x[u][i]) : a[i] * s;
+            for (int i = 0; i < 4; ++i) {
+              const float s = bf16_at(ks[u][i / 2][k / 2], k % 2);
+              x[u][i] = k ? fmaf(a[i], s, x[u][i]) : a[i] * s;
+            }
           }
           w[u].x >>= 8; w[u].y >>= 8; w[u].z >>= 8; w[u].w >>= 8;
         }
       }
+    }
+    if constexpr (FEW) {
+#pragma unroll
+      for (int u = 0; u < NP; ++u)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float s = (sums[u][0][2 * i] + sums[u][1][2 * i]) * bf16_at(ks[u][i][0], 0);
+          x[u][i] = fmaf(sums[u][0][2 * i + 1] + sums[u][1][2 * i + 1], bf16_at(ks[u][i][0], 1), s);
+          if constexpr (PAIRS == 2) x[u][i] += __shfl_xor_sync(~0u, x[u][i], 1);
+        }
     }
     // take out what some queries do not see
     uint32_t keep[NP][2];                          // halves of P that their query sees
@@ -327,37 +371,45 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         const bool s = tokens[u] & 15;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const bool a = token + 8 * i <= (s ? limit[1][0] : limit[0][0]), b = token + 8 * i <= (s ? limit[1][1] : limit[0][1]);
-          keep[u][i] = (a ? 0x0000ffffu : 0u) | (b ? 0xffff0000u : 0u);
-          if (!a) x[u][2 * i] = -INFINITY;
-          if (!b) x[u][2 * i + 1] = -INFINITY;
-          if (!a && !b)
+          bool any = false;
+          keep[u][i] = 0;
 #pragma unroll
-            for (int k = 0; k < NG / 2; ++k) vs[u][i][k] = 0;
+          for (int j = 0; j < QL; ++j) {
+            const bool sees = token + 8 * i <= (s ? limit[1][j] : limit[0][j]);
+            any = any || sees;
+            keep[u][i] |= sees ? (FEW ? ~0u : j ? 0xffff0000u : 0x0000ffffu) : 0u;
+            if (!sees) x[u][QL * i + j] = -INFINITY;
+          }
+          if (!any)
+#pragma unroll
+            for (int k = 0; k < SW; ++k) vs[u][i][k] = 0;
         }
       }
     }
 
     // renew the maxima and powers of two where they are exceeded
-    float top[2];
-    __nv_bfloat162 scale_top[NG / 2];
+    float top[QL];
+    __nv_bfloat162 scale_top[SW];
 #pragma unroll
     for (int u = 0; u < NP; ++u) {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) top[i] = u ? fmaxf(top[i], fmaxf(x[u][i], x[u][i + 2])) : fmaxf(x[u][i], x[u][i + 2]);
+      for (int i = 0; i < QL; ++i) top[i] = u ? fmaxf(top[i], fmaxf(x[u][i], x[u][i + QL])) : fmaxf(x[u][i], x[u][i + QL]);
 #pragma unroll
-      for (int k = 0; k < NG / 2; ++k) {
+      for (int k = 0; k < SW; ++k) {
         const __nv_bfloat162 s = __hmax2(as_bf162(vs[u][0][k]), as_bf162(vs[u][1][k]));
         scale_top[k] = u ? __hmax2(scale_top[k], s) : s;
       }
     }
     uint32_t over = 0;
 #pragma unroll
-    for (int k = 0; k < NG / 2; ++k) over |= __hgt2_mask(scale_top[k], ceiling[k]);
-    if (__any_sync(~0u, top[0] > limit_m[0] || top[1] > limit_m[1] || over)) {
-      float f[2];
+    for (int k = 0; k < SW; ++k) over |= __hgt2_mask(scale_top[k], ceiling[k]);
+    bool due = over;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < QL; ++i) due = due || top[i] > limit_m[i];
+    if (__any_sync(~0u, due)) {
+      float f[QL], ratio[2 * SW];
+#pragma unroll
+      for (int i = 0; i < QL; ++i) {
         float t = top[i];
 #pragma unroll
         for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
@@ -371,71 +423,87 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         l[i] *= f[i];
       }
 #pragma unroll
-      for (int k = 0; k < NG; ++k) {
-        float t = k % 2 ? __high2float(scale_top[k / 2]) : __low2float(scale_top[k / 2]), ratio = 1.f;
+      for (int k = 0; k < 2 * SW; ++k) {
+        float t = k % 2 ? __high2float(scale_top[k / 2]) : __low2float(scale_top[k / 2]);
+        // (lanes with the same columns; without FEW every lane has all groups, of tokens that one of its queries sees)
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+        for (int d = FEW ? 4 : 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+        ratio[k] = 1.f;
         if (t > (k % 2 ? __high2float(ceiling[k / 2]) : __low2float(ceiling[k / 2]))) {
           const int e = exponent_of(t);            // the largest scale becomes 2^7 .. 2^8 in P
           const float b = exact_exp2(7 - e), old = bf16_at(boost[k / 2], k % 2);
-          ratio = old > 0.f ? b / old : 0.f;
+          ratio[k] = old > 0.f ? b / old : 0.f;
           boost[k / 2] = k % 2 ? (boost[k / 2] & 0xffffu) | __float_as_uint(b) : (boost[k / 2] & 0xffff0000u) | __float_as_uint(b) >> 16;
           const __nv_bfloat16 c = __float2bfloat16_rn(exact_exp2(e + 4));
           ceiling[k / 2] = k % 2 ? __halves2bfloat162(__low2bfloat16(ceiling[k / 2]), c) : __halves2bfloat162(c, __high2bfloat16(ceiling[k / 2]));
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          acc[2 * k][i] *= f[i % 2] * ratio;
-          acc[2 * k + 1][i] *= f[i % 2] * ratio;
-          eights[k][i] *= f[i % 2] * ratio;
-        }
       }
+#pragma unroll
+      for (int n = 0; n < NK; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[n][i] *= FEW ? f[0] * ratio[i % 2] : f[i % QL] * ratio[FEW ? 0 : n / 2];
+#pragma unroll
+      for (int k = 0; k < NE; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) eights[k][i] *= FEW ? f[0] * ratio[i % 2] : f[i % QL] * ratio[FEW ? 0 : k];
     }
 
 #pragma unroll
     for (int u = 0; u < NP; ++u)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[u][i] = fast_exp2(fmaf(x[u][i], unscale[i % 2], neg_m[i % 2]));
-        l[i % 2] += x[u][i];
+      for (int i = 0; i < 2 * QL; ++i) {
+        x[u][i] = fast_exp2(fmaf(x[u][i], unscale[i % QL], neg_m[i % QL]));
+        l[i % QL] += x[u][i];
       }
     auto add_values = [&](auto some_unseen) {
 #pragma unroll
-      for (int u = 0; u < NP; ++u)
+      for (int u = 0; u < NP; ++u) {
+        // P as operands, of group k (FEW: of all groups), and with SPLIT what its rounding cut off
+        uint32_t b[SPLIT ? 2 : 1][2];
+        auto weights = [&]([[maybe_unused]] int k) {
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float w0, w1;
+            if constexpr (FEW) {
+              w0 = x[u][i] * bf16_product(vs[u][i][0], boost[0], 0);
+              w1 = x[u][i] * bf16_product(vs[u][i][0], boost[0], 1);
+            } else {
+              const float s = bf16_product(vs[u][i][k / 2], boost[k / 2], k % 2);
+              w0 = x[u][2 * i] * s;
+              w1 = x[u][2 * i + 1] * s;
+            }
+            uint32_t h = pack_half(w0, w1);
+            if constexpr (some_unseen) h &= keep[u][i];   // (0 times a NaN scale of a token that this query does not see)
+            b[0][i] = transpose8(h);
+            if constexpr (SPLIT) {
+              const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h));
+              uint32_t rest = pack_half(w0 - r.x, w1 - r.y);
+              if constexpr (some_unseen) rest &= keep[u][i];
+              b[1][i] = transpose8(rest);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < (SPLIT ? 2 : 1); ++j) mma_half(eights[FEW ? 0 : k], kEights, kEights, kEights, kEights, b[j][0], b[j][1]);
+        };
+        if constexpr (FEW) weights(0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           uint4 w = reinterpret_cast<const uint4*>(rec + u * REC + HALF + c * 512)[lane];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int k = 2 * c + half, n = 4 * c + 2 * half;
-            const float s0 = bf16_product(vs[u][0][k / 2], boost[k / 2], k % 2), s1 = bf16_product(vs[u][1][k / 2], boost[k / 2], k % 2);
-            uint32_t h0 = pack_half(x[u][0] * s0, x[u][1] * s0), h1 = pack_half(x[u][2] * s1, x[u][3] * s1);
-            if constexpr (some_unseen) {           // (0 times a NaN scale of a token that this query does not see)
-              h0 &= keep[u][0];
-              h1 &= keep[u][1];
-            }
+            if constexpr (!FEW) weights(k);
             const uint4 lo = make_uint4(w.x & 0x000f000fu, w.y & 0x000f000fu, w.z & 0x000f000fu, w.w & 0x000f000fu);
             const uint4 hi = make_uint4(w.x & 0x00f000f0u, w.y & 0x00f000f0u, w.z & 0x00f000f0u, w.w & 0x00f000f0u);
-            auto add = [&](uint32_t p0, uint32_t p1) {
-              const uint32_t b0 = transpose8(p0), b1 = transpose8(p1);
-              mma_half(acc[n], lo.x, lo.y, lo.z, lo.w, b0, b1);
-              mma_half(acc[n + 1], hi.x, hi.y, hi.z, hi.w, b0, b1);
-              mma_half(eights[k], kEights, kEights, kEights, kEights, b0, b1);
-            };
-            add(h0, h1);
-            if constexpr (SPLIT) {
-              const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h0)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h1));
-              h0 = pack_half(x[u][0] * s0 - f0.x, x[u][1] * s0 - f0.y);
-              h1 = pack_half(x[u][2] * s1 - f1.x, x[u][3] * s1 - f1.y);
-              if constexpr (some_unseen) {
-                h0 &= keep[u][0];
-                h1 &= keep[u][1];
-              }
-              add(h0, h1);
+#pragma unroll
+            for (int j = 0; j < (SPLIT ? 2 : 1); ++j) {
+              mma_half(acc[n], lo.x, lo.y, lo.z, lo.w, b[j][0], b[j][1]);
+              mma_half(acc[n + 1], hi.x, hi.y, hi.z, hi.w, b[j][0], b[j][1]);
             }
             w.x >>= 8; w.y >>= 8; w.z >>= 8; w.w >>= 8;
           }
         }
+      }
     };
     if (masked) add_values(std::true_type());
     else add_values(std::false_type());
@@ -451,22 +519,25 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   float* own = reinterpret_cast<float*>(ring);     // [queries][D]
 #pragma unroll
   for (int k = 0; k < NG; ++k) {
-    const float b = bf16_at(boost[k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
+    if (FEW && k / 2 != my_pair) continue;
+    const float b = bf16_at(boost[FEW ? 0 : k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      if (2 * t4 + i < nq)
+    for (int i = 0; i < QL; ++i)
+      if (my_query + i < nq)
 #pragma unroll
-        for (int j = 0; j < 4; ++j)                // channel g + 8 j of the group
-          own[(2 * t4 + i) * D + k * 32 + g + 8 * j] =
-              (acc[2 * k + j / 2][i + j % 2 * 2] * (j / 2 ? 0.0625f : 1.f) - eights[k][i]) * 0x1p24f * back;
+        for (int j = 0; j < 4; ++j) {              // channel g + 8 j of the group
+          const int column = FEW ? k % 2 : i;
+          own[(my_query + i) * D + k * 32 + g + 8 * j] =
+              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 0.0625f : 1.f) - eights[FEW ? 0 : k][column]) * 0x1p24f * back;
+        }
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
+  for (int i = 0; i < QL; ++i) {
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) l[i] += __shfl_xor_sync(~0u, l[i], d);
-    if (g == 0) {
-      part_m[warp][2 * t4 + i] = l[i] > 0.f || l[i] != l[i] ? -neg_m[i] : kNothing;
-      part_l[warp][2 * t4 + i] = l[i];
+    if (g == 0 && my_pair == 0) {
+      part_m[warp][my_query + i] = l[i] > 0.f || l[i] != l[i] ? -neg_m[i] : kNothing;
+      part_l[warp][my_query + i] = l[i];
     }
   }
   __syncthreads();
@@ -521,33 +592,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   }
 }
 
-template <typename T, int D, int NP> int launch(const AttnParams& p, int64_t groups, cudaStream_t stream) {
+template <typename T, int D, bool FEW, int NP> int launch(const AttnParams& p, int64_t groups, cudaStream_t stream) {
   constexpr int bytes = kWarps * kStages * NP * record_bytes(D);
-  auto kernel = cache_attn_kernel<T, D, std::is_same_v<T, __half>, NP>;
-  static thread_local bool ready[64] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess && !(dev < 64 && ready[dev])) {
-    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess && dev < 64) ready[dev] = true;
-  }
-  if (e == cudaSuccess) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(groups * p.cluster));
-    cfg.blockDim = dim3(kWarps * 32);
-    cfg.dynamicSmemBytes = bytes;
-    cfg.stream = stream;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = p.cluster;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kernel, p);
-  }
+  auto kernel = cache_attn_kernel<T, D, std::is_same_v<T, __half>, FEW, NP>;
+  static_assert(bytes + 9000 <= 48 * 1024, "shared memory that needs no opting in");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(groups * p.cluster));
+  cfg.blockDim = dim3(kWarps * 32);
+  cfg.dynamicSmemBytes = bytes;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = p.cluster;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e == cudaSuccess) return BSP_OK;
   (void)cudaGetLastError();
   return fail(BSP_ERR_CUDA, "cache attention: %s", cudaGetErrorString(e));
+}
+
+template <typename T, int D> int pick(const AttnParams& p, int64_t groups, bool few, bool many, cudaStream_t stream) {
+  constexpr int NP = 256 / D;
+  if (few) return many ? launch<T, D, true, NP>(p, groups, stream) : launch<T, D, true, 1>(p, groups, stream);
+  return many ? launch<T, D, false, NP>(p, groups, stream) : launch<T, D, false, 1>(p, groups, stream);
 }
 
 }  // namespace
@@ -602,10 +671,7 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   const bool many = granules > 16 * kWarps * p.cluster;
   if (Z > INT32_MAX / Hk / p.tiles / p.cluster) return fail(BSP_ERR_UNSUPPORTED, "cache attention: too many queries");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (many) {
-    if (dtype == BSP_F16) return D == 64 ? launch<__half, 64, 4>(p, groups, s) : launch<__half, 128, 2>(p, groups, s);
-    return D == 64 ? launch<__nv_bfloat16, 64, 4>(p, groups, s) : launch<__nv_bfloat16, 128, 2>(p, groups, s);
-  }
-  if (dtype == BSP_F16) return D == 64 ? launch<__half, 64, 1>(p, groups, s) : launch<__half, 128, 1>(p, groups, s);
-  return D == 64 ? launch<__nv_bfloat16, 64, 1>(p, groups, s) : launch<__nv_bfloat16, 128, 1>(p, groups, s);
+  const bool few = T * p.G * (D / kGroup) <= kQueries;
+  if (dtype == BSP_F16) return D == 64 ? pick<__half, 64>(p, groups, few, many, s) : pick<__half, 128>(p, groups, few, many, s);
+  return D == 64 ? pick<__nv_bfloat16, 64>(p, groups, few, many, s) : pick<__nv_bfloat16, 128>(p, groups, few, many, s);
 }
