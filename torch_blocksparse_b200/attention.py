@@ -219,7 +219,8 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         (sequences shorter than T) and queries that see nothing give zeros.  scale: head_dim ** -0.5.
 
         One kernel, without workspace, on the current stream of the cache's device; no gradient.  Lengths
-        and tables are read on the device, so that a captured call can be replayed as sequences grow."""
+        and tables are read on the device, so that a captured call can be replayed as sequences grow (the
+        first call for a layout uploads its tables: not inside a capture)."""
         cache_op = cache._op()
         key = (cache_op.heads, query.get_device(), None if self.layout is not None else pages.size(-1) * cache.page, 'decode')
         op = self._attn.get(key) or self._decode_op(key, cache, query.device)

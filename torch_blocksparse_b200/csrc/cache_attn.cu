@@ -13,7 +13,10 @@
 //   O^T = V^T P   16 channels x 16 tokens by 16 tokens x 8 queries, P = p * s for each group, so that the codes
 //                 are used as they are here too; the + 8 leaves through one product with a matrix of eights for each
 //                 group.  P comes out of S^T's accumulators by two transposes of 8 x 8 (movmatrix).
-// Eight queries (query heads that share a head of the cache, times new tokens) ride along for one.  tcgen05 has no
+// Eight queries (query heads that share a head of the cache, times new tokens) ride along for one.  Where there are so few
+// that queries times groups fit into the 8 columns (FEW: 4 queries of 64 channels, 2 of 128), a column is a (query, group):
+// q is zero outside its group, S^T comes out by groups, P of all groups is one operand with one transpose and one product of
+// eights, and a lane deals with one query and two groups' scales (592 heads x 8192 keys of 128: 138 -> 111 us).  tcgen05 has no
 // place here: its operands come from shared or tensor memory, and storing unpacked codes there would
 // cost more than the products, which use a fraction of mma.sync's rate at this width.
 //
@@ -28,10 +31,12 @@
 // queries) in turn, each through a ring of its own (cp.async, no barriers), and join their sums
 // once, in shared memory, then by sending them over the cluster, in a fixed order: results do not depend on timing.
 //
-// What bounds it now: instructions.  A granule of 128 channels takes an SM's quarter 490 cycles; loading alone takes 375 (the
-// whole of the memory's rate).  Masks, shifts, packing and maxima hold the issue port two cycles each (64 + 16 + 8 + 8 of
-// them), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one.  More warps an SM (96 or 80
-// registers) change nothing.  592 heads x sequences of 8192 keys, G = 4: bf16 138 us, 77 % of the copy rate.
+// What bounds it now.  592 heads x 8192 keys, all of a layout: bf16, 128 channels, one query each 111 us, 96 % of the copy rate
+// (fp16 85 %); four queries each 138 us, 77 %; 64 channels 72 us, 74 %.  Short of the memory's rate it is instructions: masks, shifts,
+// packing and maxima hold an SM's issue ports two cycles each (64 + 16 + 8 + 8 of them for 16 tokens of 128 channels and more
+// than two queries), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one: 490 cycles of an SM's quarter where
+// loading takes 375.  More warps an SM (96 or 80 registers) change nothing.  Short rows are bound by the chain of loads
+// (length, row, block, page, data), the launch and the join: 5 us for 9 granules a warp.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -662,10 +667,10 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   p.tiles = (T * p.G + kQueries - 1) / kQueries;
   p.scale_log2e = scale * 1.4426950408889634f;
   const int64_t groups = static_cast<int64_t>(Z) * Hk * p.tiles;
-  // CTAs of a cluster: as many as fit the SMs at once (one sequence of 12 heads, 36 blocks of 64: 8 CTAs 5.4 us, one 6.4;
-  // 8 x 16 heads: 4 CTAs 10.7 us, 8 CTAs, which do not fit, 16.5), and a granule of an average row for every warp.
-  // Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys: 107 us, one at a
-  // time 111); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 12.4 us, one at a time 10.7).
+  // CTAs of a cluster: as many as fit the SMs at once (one sequence of 12 heads, rows of up to 19 blocks of 64: 8 CTAs 5.0 us,
+  // one 6.4; 8 x 16 heads, 36 blocks: 4 CTAs 9.9 us, one 16.3, 8 CTAs, which do not fit, 14.6), and a granule of an average row
+  // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys, four
+  // queries each: 107 us, one at a time 119); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 11.3 us, one at a time 9.9).
   const int64_t granules = (static_cast<int64_t>(mt.nnz) / (static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
   p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * 148 / groups, granules / kWarps})));
   const bool many = granules > 16 * kWarps * p.cluster;

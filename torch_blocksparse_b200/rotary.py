@@ -29,7 +29,7 @@ class Rotary(_lib.WithOps):
     or BF16; any strides; the numbers of heads may differ) and returns the turned query, or query and
     key, as new tensors in their operands' memory order.  positions: int32 or int64 on the same device,
     [axes, L] or [axes, Z, L], or [L] for one axis, negative ones too; None: 0, 1, .. L - 1 on one axis.
-    Angles are exact to 2^-25 of a half turn at any position.  Both operands are differentiable (the
+    Angles are exact to 2^-25 of a half turn at any position.  (The first call on a device uploads a table: not inside a capture.)  Both operands are differentiable (the
     gradient is turned back), positions are not.
     """
 
