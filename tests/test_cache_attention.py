@@ -231,6 +231,58 @@ def test_non_finite_values_reach_those_who_see_them():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('T', [1, 5])
+def test_scales_of_either_sign_and_powers_of_two(dtype, T):
+    Z, H, L, D = 2, 2, 150, 64
+    lengths = ints(150, 77)
+    cache, pages, k, v = filled(Z, H, L, D, 32, dtype, lengths)
+    layout = layouts.dense(1, 5)
+    attn, there = SparseSelfAttention(layout=layout, block=32), torch.ones(Z, L, dtype=torch.bool)
+    q = queries(Z, 2 * H, T, D, dtype)
+    for scale in (-0.2, 0.0, 3.0, 1e-3):
+        assert_decoded(attn.decode(q, cache, pages, lengths, scale=scale), q, k, v, there, lengths, layout, 32, scale)
+    # a power of two between the query and the scale, or on the values, changes no bit
+    want = attn.decode(q, cache, pages, lengths)
+    if dtype == torch.bfloat16:
+        assert torch.equal(attn.decode(q * 2.0 ** -40, cache, pages, lengths, scale=D ** -0.5 * 2.0 ** 40), want)
+        assert torch.equal(attn.decode(q * 2.0 ** 30, cache, pages, lengths, scale=D ** -0.5 * 2.0 ** -30), want)
+        small, far = Guarded(cache.num_pages, H, D, page=32), torch.zeros(Z, dtype=torch.int32, device='cuda')
+        for shift in (2.0 ** -50, 2.0 ** 50):
+            small.write(k.to(dtype), (v * shift).to(dtype), pages, far, lengths)
+            kk, vv = small.read(pages, far, L, lengths, dtype=torch.float32)
+            assert_decoded(attn.decode(q, small, pages, lengths), q, kk, vv, there, lengths, layout, 32, D ** -0.5)
+
+
+@pytest.mark.gpu
+def test_pages_shared_by_sequences():
+    """One prompt's pages in every sequence's table (a row expanded over the batch), read only."""
+    H, L, D = 2, 100, 64
+    cache, pages, k, v = filled(1, H, L, D, 32, torch.float16, ints(L))
+    shared, lengths = pages.expand(3, -1), ints(100, 64, 33)
+    q, layout = queries(3, H, 1, D, torch.float16), layouts.dense(1, 4)
+    got = SparseSelfAttention(layout=layout, block=32).decode(q, cache, shared, lengths)
+    assert_decoded(got, q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1), torch.ones(3, L, dtype=torch.bool), lengths, layout, 32, D ** -0.5)
+    kk, _ = cache.read(shared, ints(0, 5, 50), 50, dtype=torch.float32)
+    assert torch.equal(kk[2], k[0, :, 50:]) and torch.equal(kk[1], k[0, :, 5:55])
+
+
+@pytest.mark.gpu
+def test_copies_and_pickles_of_a_cache():
+    import copy
+    import pickle
+    cache, pages, k, v = filled(1, 2, 40, 64, 16, torch.float16, ints(40))
+    plain = KVCache(cache.data.size(0), 2, 64, page=16)
+    plain.data.copy_(cache.data)
+    attn, q = SparseSelfAttention(layout=layouts.dense(1, 3), block=16), queries(1, 2, 1, 64, torch.float16)
+    want = attn.decode(q, plain, pages, ints(40))
+    for other in (copy.deepcopy(plain), pickle.loads(pickle.dumps(plain))):
+        assert torch.equal(copy.deepcopy(attn).decode(q, other, pages, ints(40)), want)
+        other.data.fill_(0)
+        assert torch.equal(attn.decode(q, plain, pages, ints(40)), want)
+
+
+@pytest.mark.gpu
 def test_zero_and_tiny_values():
     H, D = 2, 64
     cache, pages = Guarded(4, H, D), table(1, 4, 4)

@@ -216,6 +216,33 @@ def test_empty_operands_and_non_finite_values():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('order', ['contiguous', 'sequence first'])
+def test_addresses_past_32_bits(order):
+    L, H, D = (1 << 23) + 5, 3, 96                     # 2.4 G elements
+    assert L * H * D > 2 ** 31
+    rotary = Rotary(D, (16, 16))
+    x = torch.empty((1, H, L, D) if order == 'contiguous' else (L, 1, H, D), device='cuda', dtype=torch.bfloat16).normal_()
+    x = x if order == 'contiguous' else x.permute(1, 2, 0, 3)
+    positions = torch.stack([torch.arange(L, device='cuda') // 1000, torch.arange(L, device='cuda') % 1000])
+    y = rotary(x, positions=positions)
+    for at in (slice(0, 9), slice(L // 2, L // 2 + 9), slice(L - 9, L)):
+        assert_turned(y[:, :, at], rotary, x[:, :, at], positions[:, at])
+
+
+@pytest.mark.gpu
+def test_copies_and_pickles():
+    import copy
+    import pickle
+    rotary, x = Rotary(32, (8, 8), interleaved=True), operand((1, 2, 7, 32), torch.float32)
+    positions = torch.randint(0, 99, (2, 7), device='cuda')
+    want = rotary(x, positions=positions)
+    for other in (copy.deepcopy(rotary), pickle.loads(pickle.dumps(rotary))):
+        assert torch.equal(other(x, positions=positions), want)
+    rotary.interleaved = False                          # an attribute that is changed counts
+    assert_turned(rotary(x, positions=positions), rotary, x, positions)
+
+
+@pytest.mark.gpu
 def test_traced():
     rotary = Rotary(32, (8, 8))
     q, k, positions = operand((2, 3, 6, 32), torch.float32), operand((2, 1, 6, 32), torch.float32), torch.randint(0, 9, (2, 6), device='cuda')

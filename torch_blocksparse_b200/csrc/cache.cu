@@ -62,7 +62,7 @@ __device__ __forceinline__ float2 to_f2(__nv_bfloat162 v) { return __bfloat1622f
 // bits are c + 8.  max / 7 is the rounded product with 1 / 7 and one step of correction by its exact remainder, which
 // gives the rounded quotient (checked over both types' values, with the rest, by the tests).
 struct Scale {
-  float s, r;                      // r = 0: zeros, infinities, NaN, or a scale whose reciprocal a float does not hold
+  float s, r;                      // r = 0: infinities, NaN, or a scale whose reciprocal a float does not hold; zeros: any other
   uint32_t bits;
   __device__ __forceinline__ explicit Scale(float amax) {
     constexpr float kSeventh = 1.f / 7.f;
@@ -70,6 +70,7 @@ struct Scale {
     __nv_bfloat16 b = __float2bfloat16_rn(__fmaf_rn(__fmaf_rn(-7.f, q, amax), kSeventh, q));
     r = 0.f;
     if (amax > 1e-29f && amax < INFINITY) asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__bfloat162float(b)));
+    else if (amax == 0.f) r = 1.f;
     else b = amax < INFINITY ? __float2bfloat16_rn(__fdiv_rn(amax, 7.f)) : __ushort_as_bfloat16(0x7fff);
     s = __bfloat162float(b);
     bits = __bfloat16_as_ushort(b);

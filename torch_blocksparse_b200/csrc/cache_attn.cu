@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
           first = gran * kGranule + s;
           if (gran * kGranule <= (s ? last[1] : last[0])) record = static_cast<int>(p.pages.granule(z, hk, gran));
         }
+        __syncwarp();                              // (the last 32 have been read)
         const uint32_t has = __ballot_sync(~0u, record >= 0);
         if (record >= 0) listed[warp][__popc(has & ((1u << lane) - 1))] = make_int2(record, first);
         __syncwarp();
