@@ -117,7 +117,7 @@ __device__ __forceinline__ uint32_t gather_fields(const uint32_t (&pair)[4], int
   const bool hi = n & 2, odd = n & 1;               // quarters differ in lane bits 2 (hi) and 1 (odd)
   const uint32_t k0 = (hi ? w[2] : w[0]) | __shfl_xor_sync(~0u, hi ? w[0] : w[2], 4);
   const uint32_t k1 = (hi ? w[3] : w[1]) | __shfl_xor_sync(~0u, hi ? w[1] : w[3], 4);
-  return (odd ? k1 : k0) | __shfl_xor_sync(~0u, odd ? k0 : k1, 2);
+  return place_fields((odd ? k1 : k0) | __shfl_xor_sync(~0u, odd ? k0 : k1, 2));
 }
 
 // What a lane of a token writes, by the token's place j in the granule: for every K or V one word (of K) or two half words (of V),
@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_write_kernel(const __grid_c
           else encode(std::false_type());
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
+            word[h] = place_fields(word[h]);
             if (kv) asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;\n" : "+r"(word[h]));
             w[kv ? h + 2 * i : i + 2 * h] = word[h];
           }
@@ -247,19 +248,20 @@ struct ReadParams {
   int T, ctas;
 };
 
-// half (low or high of a pair) + c, in 32 bits: one instruction where a conversion and a sum are two
-__device__ __forceinline__ float add_half(uint32_t pair, int i, float c) {
+// half (low or high of a pair) * f + c, in 32 bits: one instruction where a conversion and a sum are two
+__device__ __forceinline__ float half_fma(uint32_t pair, int i, uint16_t f, float c) {
   float x;
-  if (i) asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.f16 %0, h, %2;}" : "=f"(x) : "r"(pair), "f"(c));
-  else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.f16 %0, l, %2;}" : "=f"(x) : "r"(pair), "f"(c));
+  if (i) asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; fma.rn.f32.f16 %0, h, %2, %3;}" : "=f"(x) : "r"(pair), "h"(f), "f"(c));
+  else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; fma.rn.f32.f16 %0, l, %2, %3;}" : "=f"(x) : "r"(pair), "h"(f), "f"(c));
   return x;
 }
 __device__ __forceinline__ void put2(float* p, float a, float b) { *reinterpret_cast<float2*>(p) = make_float2(a, b); }
 __device__ __forceinline__ void put2(__half* p, float a, float b) { *reinterpret_cast<__half2*>(p) = __floats2half2_rn(a, b); }
 __device__ __forceinline__ void put2(__nv_bfloat16* p, float a, float b) { *reinterpret_cast<__nv_bfloat162*>(p) = __floats2bfloat162_rn(a, b); }
 
-// Every lane takes the words that a lane of the matrix instruction would: quarter n of a word under a mask, put
-// beside the exponent of 1024 (n even) or 64 (n odd), is the half 1024 + (c + 8) or 64 + (c + 8).  K's words hold two channels
+// Every lane takes the words that a lane of the matrix instruction would: field n of a word under a mask, put
+// beside the exponent of 128, is the half 128 + (c + 8) for n even; for n odd it is (c + 8) * 2^-17 as it is, of which
+// 2^15 times less 2 makes c / 4, for scales times 4 (at most 2^127).  K's words hold two channels
 // of a token; V's hold two tokens of a channel and become the same by a transpose of 8 x 8 (movmatrix).  Rows
 // are put together in shared memory and stored 16 bytes at a time.  Against 8 channels of a token a lane, picked
 // field by field (109 instructions for 8 values): 8 sequences of up to 8192 tokens, 16 heads of 64, 63 -> 54 us; 4 of 16384 tokens,
@@ -305,12 +307,14 @@ __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_co
         uint32_t word = a == 0 ? w[kv][c].x : a == 1 ? w[kv][c].y : a == 2 ? w[kv][c].z : w[kv][c].w;
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
-          uint32_t pair = n % 2 ? (word & 0x00f000f0u) | 0x54005400u : (word & 0x000f000fu) | 0x64006400u;
+          uint32_t pair = n % 2 ? word & kHighField : (word & kLowField) | 0x58005800u;
           if (kv) asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;\n" : "+r"(pair));
           const uint32_t s2 = scale[kv][i][c];
-          const float s = __uint_as_float(n / 2 ? s2 & 0xffff0000u : s2 << 16), off = n % 2 ? -72.f : -1032.f;
-          put2(own + (g + 8 * i) * PITCH + 64 * c + 16 * n + 8 * h + 2 * t4, add_half(pair, 0, off) * s, add_half(pair, 1, off) * s);
-          if (n == 1) word >>= 8;
+          const float s = __uint_as_float(n / 2 ? s2 & 0xffff0000u : s2 << 16) * (n % 2 ? 4.f : 1.f);
+          const uint16_t f = n % 2 ? 0x7800 : 0x3c00;               // 2^15, 1
+          const float off = n % 2 ? -2.f : -136.f;
+          put2(own + (g + 8 * i) * PITCH + 64 * c + 16 * n + 8 * h + 2 * t4, half_fma(pair, 0, f, off) * s, half_fma(pair, 1, f, off) * s);
+          if (n == 1) word = swap_bytes(word);
         }
       }
     __syncwarp();

@@ -7,7 +7,7 @@
 // Bound by memory (4.5 bits a value, each read once) if the codes reach the tensor cores in few enough
 // instructions, which is what the format is for.  A warp takes 16 tokens (a granule) at a time:
 //   S^T = K q^T   m16n8k16: 16 tokens x 16 channels by 16 channels x 8 queries.  The operand is a code word
-//                 under a mask: c + 8 as a denormal half, 2^-24 each (16 * 2^-24 in the odd quarters, for which
+//                 under a mask: c + 8 as a half, times 2^-21 (2^-17 in the odd quarters, for which
 //                 q is divided by 16), exact.  The + 8 leaves through the accumulator's start, -8 * sum(q).
 //                 One multiply-add per group of 32 channels, token and query brings the scale in.
 //   O^T = V^T P   16 channels x 16 tokens by 16 tokens x 8 queries, P = p * s for each group, so that the codes
@@ -59,7 +59,7 @@ constexpr int kQueries = 8;
 constexpr int kMaxCluster = 8;
 constexpr float kNothing = -3e38f; // the maximum of no scores
 constexpr float kSlack = 4.f;      // p <= 2^4
-constexpr uint32_t kEights = 0x00080008u;        // halves 8 * 2^-24
+constexpr uint32_t kEights = 0x04000400u;        // halves 2^-14: 8 as a code in a high field
 constexpr int kNone = 0x7ffffff0;  // the token of a granule that is not there: nobody sees it
 
 struct AttnParams {
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     // |q| < 2^(e + 1); q * 2^(13 - e) < 2^14, and a sixteenth of it in the odd quarters
     const int e = exponent_of(amax);
     const float sign = p.scale_log2e > 0.f ? 1.f : p.scale_log2e < 0.f ? -1.f : p.scale_log2e;   // (scores come out scaled by > 0)
-    const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 2048.f, 0x1p-100f);          // 2^24 * 2^(e - 13)
+    const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 256.f, 0x1p-100f);           // 2^21 * 2^(e - 13)
 #pragma unroll
     for (int i = 0; i < QL; ++i) unscale[i] = __shfl_sync(~0u, down, (FEW ? my_query * NG : my_query + i) * 4);
     const float up = exact_exp2(13 - e) * sign;
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       sum += __shfl_xor_sync(~0u, sum, 2);
       const bool mine = !FEW || g % NG == k;       // (a column of another group: zeros)
       q_operand[k][lane] = mine ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(0, 0, 0, 0);
-      if (t4 == 0 && mine) reinterpret_cast<float*>(q_start[FEW ? 0 : k])[g] = sum * -0x1p-21f;
+      if (t4 == 0 && mine) reinterpret_cast<float*>(q_start[FEW ? 0 : k])[g] = sum * -0x1p-18f;
     }
   }
   __syncthreads();
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     start[1] = q_start[0][t4].y;
   }
 
-  // O^T: 16 channels each by the columns (FEW: those of their own group count); sums of P times 8 * 2^-24
+  // O^T: 16 channels each by the columns (FEW: those of their own group count); sums of P times 2^-14
   constexpr int NE = FEW ? 1 : NG;
   float acc[NK][4] = {}, eights[NE][4] = {};
   // largest score before `unscale`; that it is time for a new one; minus the largest, scaled; sums of weights
@@ -333,8 +333,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         }
 #pragma unroll
         for (int u = 0; u < NP; ++u) {
-          const uint4 lo = make_uint4(w[u].x & 0x000f000fu, w[u].y & 0x000f000fu, w[u].z & 0x000f000fu, w[u].w & 0x000f000fu);
-          const uint4 hi = make_uint4(w[u].x & 0x00f000f0u, w[u].y & 0x00f000f0u, w[u].z & 0x00f000f0u, w[u].w & 0x00f000f0u);
+          const uint4 lo = make_uint4(w[u].x & kLowField, w[u].y & kLowField, w[u].z & kLowField, w[u].w & kLowField);
+          const uint4 hi = make_uint4(w[u].x & kHighField, w[u].y & kHighField, w[u].z & kHighField, w[u].w & kHighField);
           if constexpr (FEW) {
             if (k == 0) {
               mma_half_from(sums[u][0], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y, start[0], start[1]);
@@ -353,7 +353,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
               x[u][i] = k ? fmaf(a[i], s, x[u][i]) : a[i] * s;
             }
           }
-          w[u].x >>= 8; w[u].y >>= 8; w[u].z >>= 8; w[u].w >>= 8;
+          if (half == 0) w[u] = make_uint4(swap_bytes(w[u].x), swap_bytes(w[u].y), swap_bytes(w[u].z), swap_bytes(w[u].w));
         }
       }
     }
@@ -499,14 +499,14 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
           for (int half = 0; half < 2; ++half) {
             const int k = 2 * c + half, n = 4 * c + 2 * half;
             if constexpr (!FEW) weights(k);
-            const uint4 lo = make_uint4(w.x & 0x000f000fu, w.y & 0x000f000fu, w.z & 0x000f000fu, w.w & 0x000f000fu);
-            const uint4 hi = make_uint4(w.x & 0x00f000f0u, w.y & 0x00f000f0u, w.z & 0x00f000f0u, w.w & 0x00f000f0u);
+            const uint4 lo = make_uint4(w.x & kLowField, w.y & kLowField, w.z & kLowField, w.w & kLowField);
+            const uint4 hi = make_uint4(w.x & kHighField, w.y & kHighField, w.z & kHighField, w.w & kHighField);
 #pragma unroll
             for (int j = 0; j < (SPLIT ? 2 : 1); ++j) {
               mma_half(acc[n], lo.x, lo.y, lo.z, lo.w, b[j][0], b[j][1]);
               mma_half(acc[n + 1], hi.x, hi.y, hi.z, hi.w, b[j][0], b[j][1]);
             }
-            w.x >>= 8; w.y >>= 8; w.z >>= 8; w.w >>= 8;
+            if (half == 0) w = make_uint4(swap_bytes(w.x), swap_bytes(w.y), swap_bytes(w.z), swap_bytes(w.w));
           }
         }
       }
@@ -534,7 +534,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         for (int j = 0; j < 4; ++j) {              // channel g + 8 j of the group
           const int column = FEW ? k % 2 : i;
           own[(my_query + i) * D + k * 32 + g + 8 * j] =
-              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 0.0625f : 1.f) - eights[FEW ? 0 : k][column]) * 0x1p24f * back;
+              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 1.f : 16.f) - eights[FEW ? 0 : k][column]) * 0x1p17f * back;
         }
   }
 #pragma unroll
