@@ -181,6 +181,28 @@ def test_scales_and_scores_that_grow_along_the_row(dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('dtype', DTYPES)
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('L', [2, 3, 17, 64, 200])
+@pytest.mark.parametrize('G', [1, 8])
+def test_one_value_outweighs_the_others(dtype, D, L, G):
+    """Values of very different size, by token and by channel: small results beside large terms that carry the codes' offset."""
+    Z, H = 8, 4
+    g = torch.Generator(device='cuda').manual_seed(L)
+    def randn(*s): return torch.randn(s, generator=g, device='cuda')
+    k = randn(Z, H, L, D).to(dtype)
+    v = (randn(Z, H, L, D) * torch.exp2(5 * randn(Z, H, L, 1)) * torch.exp2(3 * randn(Z, H, L, D))).clamp(-30000, 30000).to(dtype)
+    slots = -(-L // 64)
+    cache, pages = Guarded(Z * slots, H, D), table(Z, slots, Z * slots)
+    zero = torch.zeros(Z, dtype=torch.int32, device='cuda')
+    cache.write(k, v, pages, zero)
+    kk, vv = cache.read(pages, zero, L, dtype=torch.float32)
+    q, layout = (randn(Z, H * G, 1, D) * 0.01).to(dtype), layouts.dense(1, 4)
+    got = SparseSelfAttention(layout=layout, block=64).decode(q, cache, pages, zero + L)
+    assert_decoded(got, q, kk, vv, torch.ones(Z, L, dtype=torch.bool), zero + L, layout, 64, D ** -0.5)
+
+
+@pytest.mark.gpu
 def test_missing_pages_lengths_behind_the_layout_and_the_table():
     Z, H, L, D, page = 4, 2, 256, 64, 32
     lengths = ints(256, 200, 300, 256)
