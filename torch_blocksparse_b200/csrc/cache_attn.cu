@@ -13,10 +13,9 @@
 //   O^T = V^T P   16 channels x 16 tokens by 16 tokens x 8 queries, P = p * s for each group, so that the codes
 //                 are used as they are here too; the + 8 leaves through one product with a matrix of eights for each
 //                 group.  P comes out of S^T's accumulators by two transposes of 8 x 8 (movmatrix).
-// Eight queries (query heads that share a head of the cache, times new tokens) ride along for one.  Where there are so few
-// that queries times groups fit into the 8 columns (FEW: 4 queries of 64 channels, 2 of 128), a column is a (query, group):
-// q is zero outside its group, S^T comes out by groups, P of all groups is one operand with one transpose and one product of
-// eights, and a lane deals with one query and two groups' scales (592 heads x 8192 keys of 128: 138 -> 111 us).  tcgen05 has no
+// Eight queries (query heads that share a head of the cache, times new tokens) ride along for one.  Where there are at most four,
+// or two of 128 channels, a column is a (query, group) of GC groups: q is zero outside its group, S^T comes out by groups, P of GC
+// groups is one operand with one transpose and one product of eights, and a lane deals with one query.  tcgen05 has no
 // place here: its operands come from shared or tensor memory, and storing unpacked codes there would
 // cost more than the products, which use a fraction of mma.sync's rate at this width.
 //
@@ -31,12 +30,12 @@
 // queries) in turn, each through a ring of its own (cp.async, no barriers), and join their sums
 // once, in shared memory, then by sending them over the cluster, in a fixed order: results do not depend on timing.
 //
-// What bounds it now.  592 heads x 8192 keys, all of a layout: bf16, 128 channels, one query each 111 us, 96 % of the copy rate
-// (fp16 85 %); four queries each 138 us, 77 %; 64 channels 72 us, 74 %.  Short of the memory's rate it is instructions: masks, shifts,
-// packing and maxima hold an SM's issue ports two cycles each (64 + 16 + 8 + 8 of them for 16 tokens of 128 channels and more
-// than two queries), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one: 490 cycles of an SM's quarter where
-// loading takes 375.  More warps an SM (96 or 80 registers) change nothing.  Short rows are bound by the chain of loads
-// (length, row, block, page, data), the launch and the join: 5 us for 9 granules a warp.
+// What bounds it now.  592 heads x 8192 keys, all of a layout, bf16: 128 channels, one query each 111 us, 96 % of the copy rate, four
+// 121 us, 88 %, eight 140 us, 77 %; 64 channels 70 us, 76 % (fp16: 85, 75 and 67 % with one, four, and one of 64).  Short of the memory's
+// rate it is instructions: masks, permutations, packing and maxima hold an SM's issue ports two cycles each (for 16 tokens of 128
+// channels and eight queries 64 + 16 + 8 + 8 of them), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one:
+// 490 cycles of an SM's quarter where loading takes 375.  More warps an SM (96 or 80 registers) change nothing.  Short rows are bound by
+// the chain of loads (length, row, block, page, data), the launch and the join: 5 us for 5 granules a warp.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -115,12 +114,13 @@ __device__ __forceinline__ float bf16_product(uint32_t pair, uint32_t other, int
 }
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
 
-template <typename T, int D, bool SPLIT, bool FEW, int NP>
+template <typename T, int D, bool SPLIT, int GC, int NP>
 __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __grid_constant__ AttnParams p) {
   constexpr int REC = record_bytes(D), HALF = REC / 2, STAGE = NP * REC, NC = D / 64, NG = D / kGroup, NK = D / 16;
-  // What a lane deals with: queries, and for each token pairs of groups of channels.  Two queries and all groups; with FEW, where
-  // queries x groups fit into 8, the columns of the products are (query, group) and a lane has one query and two groups.
-  constexpr int PAIRS = NG / 2, QL = FEW ? 1 : 2, SW = FEW ? 1 : PAIRS;
+  // Columns of the products: 8 / GC queries by GC groups of channels.  q is zero in a column outside its group, so that a
+  // column's sums over GC groups of channels (a set) belong to one of them.  A lane has columns 2 t4 and 2 t4 + 1: two queries and
+  // all groups (GC = 1), or QL = 1 query and two groups of each set, whose scales are SW words for each of its tokens.
+  constexpr int SETS = NG / GC, QL = GC == 1 ? 2 : 1, SW = GC == 4 ? 1 : NG / 2;
   extern __shared__ __align__(16) uint8_t smem[];
   __shared__ uint4 q_operand[NG][32];              // of both quarters of a group, by lane
   __shared__ float2 q_start[NG][4];                // by pair of queries
@@ -129,8 +129,8 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   __shared__ float inbox[kQueries * D + kMaxCluster], inbox_m[kMaxCluster][kQueries], inbox_l[kMaxCluster][kQueries];
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   uint8_t* ring = smem + warp * (kStages * STAGE);
-  const int my_query = FEW ? t4 / PAIRS : 2 * t4, my_pair = FEW ? t4 % PAIRS : 0;   // the first of them
-  const int q_column = FEW ? g / NG : g;           // the query of column g of the products
+  const int my_query = 2 * t4 / GC, my_word = GC == 4 ? t4 % 2 : 0;
+  const int q_column = g / GC;                     // the query of column g
 
   if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n");   // (this CTA runs: others may write here)
 
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 
   // ---- q as operands: halves scaled by a power of two, and what the codes' offset adds up to; one group of 32
   // channels a warp, kept in shared memory (registers are what limits the warps of an SM)
-  float unscale[QL], start[2];
+  float unscale[QL];
   {
     auto pair_at = [&](int n, int i) {
       if constexpr (std::is_same_v<T, __half>) return __half22float2(*reinterpret_cast<const __half2*>(&qraw[n][i]));
@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     const float sign = p.scale_log2e > 0.f ? 1.f : p.scale_log2e < 0.f ? -1.f : p.scale_log2e;   // (scores come out scaled by > 0)
     const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 256.f, 0x1p-100f);           // 2^21 * 2^(e - 13)
 #pragma unroll
-    for (int i = 0; i < QL; ++i) unscale[i] = __shfl_sync(~0u, down, (FEW ? my_query * NG : my_query + i) * 4);
+    for (int i = 0; i < QL; ++i) unscale[i] = __shfl_sync(~0u, down, (GC == 1 ? my_query + i : my_query * GC) * 4);
     const float up = exact_exp2(13 - e) * sign;
 #pragma unroll
     for (int k = 0; k < NG; ++k) {
@@ -268,20 +268,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       }
       sum += __shfl_xor_sync(~0u, sum, 1);
       sum += __shfl_xor_sync(~0u, sum, 2);
-      const bool mine = !FEW || g % NG == k;       // (a column of another group: zeros)
+      const bool mine = g % GC == k % GC;          // (a column of another group: zeros)
       q_operand[k][lane] = mine ? make_uint4(h[0], h[1], h[2], h[3]) : make_uint4(0, 0, 0, 0);
-      if (t4 == 0 && mine) reinterpret_cast<float*>(q_start[FEW ? 0 : k])[g] = sum * -0x1p-18f;
+      if (t4 == 0 && mine) reinterpret_cast<float*>(q_start[k / GC])[g] = sum * -0x1p-18f;
     }
   }
   __syncthreads();
-  if constexpr (FEW) {
-    start[0] = q_start[0][t4].x;
-    start[1] = q_start[0][t4].y;
-  }
 
-  // O^T: 16 channels each by the columns (FEW: those of their own group count); sums of P times 2^-14
-  constexpr int NE = FEW ? 1 : NG;
-  float acc[NK][4] = {}, eights[NE][4] = {};
+  // O^T: 16 channels each by the columns (those of their own group count); sums of P times 2^-14
+  float acc[NK][4] = {}, eights[SETS][4] = {};
   // largest score before `unscale`; that it is time for a new one; minus the largest, scaled; sums of weights
   float m[QL], limit_m[QL], neg_m[QL], l[QL];
 #pragma unroll
@@ -314,10 +309,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int k = 0; k < SW; ++k) {
-          ks[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + 8 * D)[(g + 8 * i) * PAIRS + my_pair + k];
-          vs[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + HALF + 8 * D)[(g + 8 * i) * PAIRS + my_pair + k];
+          ks[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + 8 * D)[(g + 8 * i) * (NG / 2) + my_word + k];
+          vs[u][i][k] = reinterpret_cast<const uint32_t*>(rec + u * REC + HALF + 8 * D)[(g + 8 * i) * (NG / 2) + my_word + k];
         }
-    float sums[NP][2][4];                          // FEW: even and odd quarters, by (query, group)
+    float a[NP][4], a_odd[NP][4];                  // a set's sums; GC = 4: of the odd quarters
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
       uint4 w[NP];
@@ -327,45 +322,36 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       for (int half = 0; half < 2; ++half) {
         const int k = 2 * c + half;
         const uint4 qf = q_operand[k][lane];
-        if constexpr (!FEW) {
-          start[0] = q_start[k][t4].x;
-          start[1] = q_start[k][t4].y;
-        }
+        const float2 start = q_start[k / GC][t4];
 #pragma unroll
         for (int u = 0; u < NP; ++u) {
           const uint4 lo = make_uint4(w[u].x & kLowField, w[u].y & kLowField, w[u].z & kLowField, w[u].w & kLowField);
           const uint4 hi = make_uint4(w[u].x & kHighField, w[u].y & kHighField, w[u].z & kHighField, w[u].w & kHighField);
-          if constexpr (FEW) {
-            if (k == 0) {
-              mma_half_from(sums[u][0], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y, start[0], start[1]);
-              mma_half_from(sums[u][1], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w, 0.f, 0.f);
-            } else {
-              mma_half(sums[u][0], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y);
-              mma_half(sums[u][1], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w);
-            }
-          } else {
-            float a[4];
-            mma_half_from(a, lo.x, lo.y, lo.z, lo.w, qf.x, qf.y, start[0], start[1]);
-            mma_half(a, hi.x, hi.y, hi.z, hi.w, qf.z, qf.w);
+          if (k % GC) mma_half(a[u], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y);
+          else mma_half_from(a[u], lo.x, lo.y, lo.z, lo.w, qf.x, qf.y, start.x, start.y);
+          if (GC < 4) mma_half(a[u], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w);
+          else if (k) mma_half(a_odd[u], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w);
+          else mma_half_from(a_odd[u], hi.x, hi.y, hi.z, hi.w, qf.z, qf.w, 0.f, 0.f);
+          if constexpr (GC == 1) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float s = bf16_at(ks[u][i / 2][k / 2], k % 2);
-              x[u][i] = k ? fmaf(a[i], s, x[u][i]) : a[i] * s;
+              x[u][i] = k ? fmaf(a[u][i], s, x[u][i]) : a[u][i] * s;
+            }
+          } else if (k % GC == GC - 1) {
+            const int word = GC == 4 ? 0 : c;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const float s0 = bf16_at(ks[u][i][word], 0), s1 = bf16_at(ks[u][i][word], 1);
+              const float a0 = GC == 4 ? a[u][2 * i] + a_odd[u][2 * i] : a[u][2 * i];
+              const float a1 = GC == 4 ? a[u][2 * i + 1] + a_odd[u][2 * i + 1] : a[u][2 * i + 1];
+              x[u][i] = fmaf(a1, s1, word ? fmaf(a0, s0, x[u][i]) : a0 * s0);
+              if constexpr (GC == 4) x[u][i] += __shfl_xor_sync(~0u, x[u][i], 1);   // (the query's other two groups)
             }
           }
           if (half == 0) w[u] = make_uint4(swap_bytes(w[u].x), swap_bytes(w[u].y), swap_bytes(w[u].z), swap_bytes(w[u].w));
         }
       }
-    }
-    if constexpr (FEW) {
-#pragma unroll
-      for (int u = 0; u < NP; ++u)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const float s = (sums[u][0][2 * i] + sums[u][1][2 * i]) * bf16_at(ks[u][i][0], 0);
-          x[u][i] = fmaf(sums[u][0][2 * i + 1] + sums[u][1][2 * i + 1], bf16_at(ks[u][i][0], 1), s);
-          if constexpr (PAIRS == 2) x[u][i] += __shfl_xor_sync(~0u, x[u][i], 1);
-        }
     }
     // take out what some queries do not see
     uint32_t keep[NP][2];                          // halves of P that their query sees
@@ -383,7 +369,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
           for (int j = 0; j < QL; ++j) {
             const bool sees = token + 8 * i <= (s ? limit[1][j] : limit[0][j]);
             any = any || sees;
-            keep[u][i] |= sees ? (FEW ? ~0u : j ? 0xffff0000u : 0x0000ffffu) : 0u;
+            keep[u][i] |= sees ? (GC > 1 ? ~0u : j ? 0xffff0000u : 0x0000ffffu) : 0u;
             if (!sees) x[u][QL * i + j] = -INFINITY;
           }
           if (!any)
@@ -431,9 +417,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 #pragma unroll
       for (int k = 0; k < 2 * SW; ++k) {
         float t = k % 2 ? __high2float(scale_top[k / 2]) : __low2float(scale_top[k / 2]);
-        // (lanes with the same columns; without FEW every lane has all groups, of tokens that one of its queries sees)
+        // (lanes with the same columns; with GC = 1 every lane has all groups, of tokens that one of its queries sees)
 #pragma unroll
-        for (int d = FEW ? 4 : 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+        for (int d = GC > 1 ? 4 : 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
         ratio[k] = 1.f;
         if (t > (k % 2 ? __high2float(ceiling[k / 2]) : __low2float(ceiling[k / 2]))) {
           const int e = exponent_of(t);            // the largest scale becomes 2^7 .. 2^8 in P
@@ -447,11 +433,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 #pragma unroll
       for (int n = 0; n < NK; ++n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] *= FEW ? f[0] * ratio[i % 2] : f[i % QL] * ratio[FEW ? 0 : n / 2];
+        for (int i = 0; i < 4; ++i) acc[n][i] *= f[i % QL] * ratio[GC == 1 ? n / 2 : GC == 2 ? n / 4 * 2 + i % 2 : i % 2];
 #pragma unroll
-      for (int k = 0; k < NE; ++k)
+      for (int k = 0; k < SETS; ++k)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) eights[k][i] *= FEW ? f[0] * ratio[i % 2] : f[i % QL] * ratio[FEW ? 0 : k];
+        for (int i = 0; i < 4; ++i) eights[k][i] *= f[i % QL] * ratio[GC == 1 ? k : GC == 2 ? 2 * k + i % 2 : i % 2];
     }
 
 #pragma unroll
@@ -464,15 +450,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     auto add_values = [&](auto some_unseen) {
 #pragma unroll
       for (int u = 0; u < NP; ++u) {
-        // P as operands, of group k (FEW: of all groups), and with SPLIT what its rounding cut off
+        // P as operands, of the k-th set, and with SPLIT what its rounding cut off
         uint32_t b[SPLIT ? 2 : 1][2];
-        auto weights = [&]([[maybe_unused]] int k) {
+        auto weights = [&](int k) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
             float w0, w1;
-            if constexpr (FEW) {
-              w0 = x[u][i] * bf16_product(vs[u][i][0], boost[0], 0);
-              w1 = x[u][i] * bf16_product(vs[u][i][0], boost[0], 1);
+            if constexpr (GC > 1) {
+              w0 = x[u][i] * bf16_product(vs[u][i][k], boost[k], 0);
+              w1 = x[u][i] * bf16_product(vs[u][i][k], boost[k], 1);
             } else {
               const float s = bf16_product(vs[u][i][k / 2], boost[k / 2], k % 2);
               w0 = x[u][2 * i] * s;
@@ -489,16 +475,15 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
             }
           }
 #pragma unroll
-          for (int j = 0; j < (SPLIT ? 2 : 1); ++j) mma_half(eights[FEW ? 0 : k], kEights, kEights, kEights, kEights, b[j][0], b[j][1]);
+          for (int j = 0; j < (SPLIT ? 2 : 1); ++j) mma_half(eights[k], kEights, kEights, kEights, kEights, b[j][0], b[j][1]);
         };
-        if constexpr (FEW) weights(0);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
           uint4 w = reinterpret_cast<const uint4*>(rec + u * REC + HALF + c * 512)[lane];
 #pragma unroll
           for (int half = 0; half < 2; ++half) {
             const int k = 2 * c + half, n = 4 * c + 2 * half;
-            if constexpr (!FEW) weights(k);
+            if (k % GC == 0) weights(k / GC);
             const uint4 lo = make_uint4(w.x & kLowField, w.y & kLowField, w.z & kLowField, w.w & kLowField);
             const uint4 hi = make_uint4(w.x & kHighField, w.y & kHighField, w.z & kHighField, w.w & kHighField);
 #pragma unroll
@@ -525,23 +510,23 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   float* own = reinterpret_cast<float*>(ring);     // [queries][D]
 #pragma unroll
   for (int k = 0; k < NG; ++k) {
-    if (FEW && k / 2 != my_pair) continue;
-    const float b = bf16_at(boost[FEW ? 0 : k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
+    if (GC == 4 && k / 2 != my_word) continue;
+    const float b = bf16_at(boost[GC == 4 ? 0 : k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
 #pragma unroll
     for (int i = 0; i < QL; ++i)
       if (my_query + i < nq)
 #pragma unroll
         for (int j = 0; j < 4; ++j) {              // channel g + 8 j of the group
-          const int column = FEW ? k % 2 : i;
+          const int column = GC > 1 ? k % 2 : i;
           own[(my_query + i) * D + k * 32 + g + 8 * j] =
-              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 1.f : 16.f) - eights[FEW ? 0 : k][column]) * 0x1p17f * back;
+              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 1.f : 16.f) - eights[k / GC][column]) * 0x1p17f * back;
         }
   }
 #pragma unroll
   for (int i = 0; i < QL; ++i) {
 #pragma unroll
     for (int d = 4; d < 32; d *= 2) l[i] += __shfl_xor_sync(~0u, l[i], d);
-    if (g == 0 && my_pair == 0) {
+    if (g == 0 && my_word == 0) {
       part_m[warp][my_query + i] = l[i] > 0.f || l[i] != l[i] ? -neg_m[i] : kNothing;
       part_l[warp][my_query + i] = l[i];
     }
@@ -598,9 +583,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   }
 }
 
-template <typename T, int D, bool FEW, int NP> int launch(const AttnParams& p, int64_t groups, cudaStream_t stream) {
+template <typename T, int D, int GC, int NP> int launch(const AttnParams& p, int64_t groups, cudaStream_t stream) {
   constexpr int bytes = kWarps * kStages * NP * record_bytes(D);
-  auto kernel = cache_attn_kernel<T, D, std::is_same_v<T, __half>, FEW, NP>;
+  auto kernel = cache_attn_kernel<T, D, std::is_same_v<T, __half>, GC, NP>;
   static_assert(bytes + 9000 <= 48 * 1024, "shared memory that needs no opting in");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(groups * p.cluster));
@@ -619,10 +604,15 @@ template <typename T, int D, bool FEW, int NP> int launch(const AttnParams& p, i
   return fail(BSP_ERR_CUDA, "cache attention: %s", cudaGetErrorString(e));
 }
 
-template <typename T, int D> int pick(const AttnParams& p, int64_t groups, bool few, bool many, cudaStream_t stream) {
-  constexpr int NP = 256 / D;
-  if (few) return many ? launch<T, D, true, NP>(p, groups, stream) : launch<T, D, true, 1>(p, groups, stream);
-  return many ? launch<T, D, false, NP>(p, groups, stream) : launch<T, D, false, 1>(p, groups, stream);
+template <typename T, int D, int GC> int pick(const AttnParams& p, int64_t groups, bool many, cudaStream_t stream) {
+  return many ? launch<T, D, GC, 256 / D>(p, groups, stream) : launch<T, D, GC, 1>(p, groups, stream);
+}
+// As many groups of channels beside the queries in the products' columns as there are places (592 heads x 8192 keys of 128,
+// bf16: one query with 4 groups 111 us, with 2 120, with 1 138; four queries with 2 groups 121, with 1 138).
+template <typename T, int D> int pick(const AttnParams& p, int64_t groups, int queries, bool many, cudaStream_t stream) {
+  if constexpr (D == 128)
+    if (queries <= 2) return pick<T, D, 4>(p, groups, many, stream);
+  return queries <= 4 ? pick<T, D, 2>(p, groups, many, stream) : pick<T, D, 1>(p, groups, many, stream);
 }
 
 }  // namespace
@@ -670,14 +660,14 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   const int64_t groups = static_cast<int64_t>(Z) * Hk * p.tiles;
   // CTAs of a cluster: as many as fit the SMs at once (one sequence of 12 heads, rows of up to 19 blocks of 64: 8 CTAs 5.0 us,
   // one 6.4; 8 x 16 heads, 36 blocks: 4 CTAs 9.9 us, one 16.3, 8 CTAs, which do not fit, 14.6), and a granule of an average row
-  // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys, four
+  // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys, eight
   // queries each: 107 us, one at a time 119); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 11.3 us, one at a time 9.9).
   const int64_t granules = (static_cast<int64_t>(mt.nnz) / (static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
   p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * 148 / groups, granules / kWarps})));
   const bool many = granules > 16 * kWarps * p.cluster;
   if (Z > INT32_MAX / Hk / p.tiles / p.cluster) return fail(BSP_ERR_UNSUPPORTED, "cache attention: too many queries");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool few = T * p.G * (D / kGroup) <= kQueries;
-  if (dtype == BSP_F16) return D == 64 ? pick<__half, 64>(p, groups, few, many, s) : pick<__half, 128>(p, groups, few, many, s);
-  return D == 64 ? pick<__nv_bfloat16, 64>(p, groups, few, many, s) : pick<__nv_bfloat16, 128>(p, groups, few, many, s);
+  const int queries = T * p.G;
+  if (dtype == BSP_F16) return D == 64 ? pick<__half, 64>(p, groups, queries, many, s) : pick<__half, 128>(p, groups, queries, many, s);
+  return D == 64 ? pick<__nv_bfloat16, 64>(p, groups, queries, many, s) : pick<__nv_bfloat16, 128>(p, groups, queries, many, s);
 }
