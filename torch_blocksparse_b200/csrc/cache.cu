@@ -264,8 +264,8 @@ __device__ __forceinline__ void put2(__nv_bfloat16* p, float a, float b) { *rein
 // 2^15 times less 2 makes c / 4, for scales times 4 (at most 2^127).  K's words hold two channels
 // of a token; V's hold two tokens of a channel and become the same by a transpose of 8 x 8 (movmatrix).  Rows
 // are put together in shared memory and stored 16 bytes at a time.  Against 8 channels of a token a lane, picked
-// field by field (109 instructions for 8 values): 8 sequences of up to 8192 tokens, 16 heads of 64, 63 -> 54 us; 4 of 16384 tokens,
-// 16 heads of 128, 112 -> 104 us, 97 % of the copy rate.
+// field by field (109 instructions for 8 values): 8 sequences of up to 8192 tokens, 16 heads of 64, 63 -> 55 us; 4 of 16384 tokens,
+// 16 heads of 128, 112 -> 105 us, 95 % of the copy rate.
 template <typename T, int D>
 __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_constant__ ReadParams p) {
   constexpr int REC = record_bytes(D), HALF = REC / 2, NC = D / 64, NG = D / kGroup;
@@ -299,7 +299,15 @@ __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_co
 #pragma unroll
   for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
-    for (int c = 0; c < NC; ++c)
+    for (int c = 0; c < NC; ++c) {
+      float s[2][4];                                 // by token half and field
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i][0] = __uint_as_float(scale[kv][i][c] << 16);
+        s[i][2] = __uint_as_float(scale[kv][i][c] & 0xffff0000u);
+        s[i][1] = 4.f * s[i][0];
+        s[i][3] = 4.f * s[i][2];
+      }
 #pragma unroll
       for (int a = 0; a < 4; ++a) {
         // K: token half a % 2, channel half a / 2; V: the other way round
@@ -309,14 +317,13 @@ __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_co
         for (int n = 0; n < 4; ++n) {
           uint32_t pair = n % 2 ? word & kHighField : (word & kLowField) | 0x58005800u;
           if (kv) asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;\n" : "+r"(pair));
-          const uint32_t s2 = scale[kv][i][c];
-          const float s = __uint_as_float(n / 2 ? s2 & 0xffff0000u : s2 << 16) * (n % 2 ? 4.f : 1.f);
           const uint16_t f = n % 2 ? 0x7800 : 0x3c00;               // 2^15, 1
           const float off = n % 2 ? -2.f : -136.f;
-          put2(own + (g + 8 * i) * PITCH + 64 * c + 16 * n + 8 * h + 2 * t4, half_fma(pair, 0, f, off) * s, half_fma(pair, 1, f, off) * s);
+          put2(own + (g + 8 * i) * PITCH + 64 * c + 16 * n + 8 * h + 2 * t4, half_fma(pair, 0, f, off) * s[i][n], half_fma(pair, 1, f, off) * s[i][n]);
           if (n == 1) word = swap_bytes(word);
         }
       }
+    }
     __syncwarp();
     T* y = static_cast<T*>(p.y[kv]) + static_cast<int64_t>(z) * p.sz[kv] + head * p.sh[kv];
     constexpr int PER = 16 / sizeof(T), PIECES = D / PER, ROWS = 32 / PIECES;
