@@ -437,6 +437,34 @@ def test_empty_calls():
     assert not bool(attn.decode(queries(2, 2, 1, 64, torch.float16), cache, pages[:, :0], ints(40, 7)).any())
 
 
+@pytest.mark.gpu
+def test_calls_one_after_the_other_see_each_other():
+    """Nothing waits between them: every call finds what the calls before it have left, other operations among them."""
+    from tests.test_cache import same, stands_for
+    Z, H, D, n = 8, 4, 64, 300
+    cache, pages = Guarded(Z * 5, H, D), table(Z, 5, Z * 5)
+    attn, rotary = SparseSelfAttention(layout=layouts.dense(1, 5), block=64), Rotary(D)
+    base, start = tokens(Z, H, 1, D, torch.float16), torch.zeros(Z, dtype=torch.int32, device='cuda')
+    got, keys, outs, wants = [], [], [], []
+    for i in range(n):
+        k = rotary(base * (1 + i % 7), positions=start[:1] + i)
+        cache.write(k, k, pages, start)
+        keys.append(k)
+        got.append(cache.read(pages, start, 1, dtype=torch.float32)[0])
+        start.add_(1)
+        outs.append(attn.decode(k, cache, pages, start))
+        k = k + 0                                       # (memory of earlier results is used again)
+    torch.cuda.synchronize()
+    again = torch.zeros_like(start)
+    for i in range(n):
+        assert same(got[i], stands_for(keys[i])), i
+        again.add_(1)
+        if i % 37 == 0 or i == n - 1:
+            wants.append(attn.decode(keys[i], cache, pages, again))
+            torch.cuda.synchronize()
+            assert torch.equal(wants[-1], outs[i]), i
+
+
 # ---- refusals ----------------------------------------------------------------------------------
 def test_the_library_rejects_bad_arguments():
     L = _lib.lib()

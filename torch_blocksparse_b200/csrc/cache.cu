@@ -13,6 +13,7 @@
 
 #include "cache.cuh"
 #include "common.h"
+#include "launch.cuh"
 #include "tile.cuh"
 
 namespace bsp {
@@ -142,6 +143,7 @@ template <typename T, int D, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32) cache_write_kernel(const __grid_constant__ WriteParams p) {
   constexpr int REC = record_bytes(D);
   __shared__ __align__(16) T rows[kWarps][kGranule * (D + 8)];
+  wait_for_earlier_kernels();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   // (a CTA's warps share a head: their number is found with one division of 32 bits for all)
   const uint32_t zh = blockIdx.x / static_cast<uint32_t>(p.ctas), z = zh / static_cast<uint32_t>(p.pages.heads);
@@ -271,6 +273,7 @@ __global__ void __launch_bounds__(kWarps * 32) cache_read_kernel(const __grid_co
   constexpr int REC = record_bytes(D), HALF = REC / 2, NC = D / 64, NG = D / kGroup;
   constexpr int PITCH = D + 32 / static_cast<int>(sizeof(T)) / (sizeof(T) == 4 ? 1 : 2);   // rows 4 (8: FP32) banks apart
   __shared__ __align__(16) T tile[kWarps][kGranule * PITCH];
+  wait_for_earlier_kernels();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t4 = lane % 4;
   // (a CTA's warps share a head: their number is found with one division of 32 bits for all)
   const uint32_t zh = blockIdx.x / static_cast<uint32_t>(p.ctas), z = zh / static_cast<uint32_t>(p.pages.heads);
@@ -364,20 +367,15 @@ int grid_of(const char* what, int Z, int H, int T, unsigned* grid, int* warps, i
   return BSP_OK;
 }
 
-int launched(const char* what) {
-  const cudaError_t e = cudaGetLastError();
+int launched(const char* what, cudaError_t e) {
   return e == cudaSuccess ? BSP_OK : fail(BSP_ERR_CUDA, "%s: %s", what, cudaGetErrorString(e));
 }
 
 template <typename T, int D> int write(const WriteParams& p, bool vec, unsigned grid, int warps, cudaStream_t s) {
-  if (vec) cache_write_kernel<T, D, true><<<grid, warps * 32, 0, s>>>(p);
-  else cache_write_kernel<T, D, false><<<grid, warps * 32, 0, s>>>(p);
-  return launched("cache write");
+  return launched("cache write", launch_kernel(vec ? cache_write_kernel<T, D, true> : cache_write_kernel<T, D, false>, grid, warps * 32, 0, s, p));
 }
 template <typename T> int read(const ReadParams& p, int D, unsigned grid, int warps, cudaStream_t s) {
-  if (D == 64) cache_read_kernel<T, 64><<<grid, warps * 32, 0, s>>>(p);
-  else cache_read_kernel<T, 128><<<grid, warps * 32, 0, s>>>(p);
-  return launched("cache read");
+  return launched("cache read", launch_kernel(D == 64 ? cache_read_kernel<T, 64> : cache_read_kernel<T, 128>, grid, warps * 32, 0, s, p));
 }
 
 }  // namespace

@@ -44,6 +44,7 @@
 
 #include "cache.cuh"
 #include "common.h"
+#include "launch.cuh"
 #include "tile.cuh"
 
 namespace bsp {
@@ -132,6 +133,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   const int my_query = 2 * t4 / GC, my_word = GC == 4 ? t4 % 2 : 0;
   const int q_column = g / GC;                     // the query of column g
 
+  wait_for_earlier_kernels();
   if (p.cluster > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;\n");   // (this CTA runs: others may write here)
 
   // ---- which queries
@@ -587,20 +589,8 @@ template <typename T, int D, int GC, int NP> int launch(const AttnParams& p, int
   constexpr int bytes = kWarps * kStages * NP * record_bytes(D);
   auto kernel = cache_attn_kernel<T, D, std::is_same_v<T, __half>, GC, NP>;
   static_assert(bytes + 9000 <= 48 * 1024, "shared memory that needs no opting in");
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>(groups * p.cluster));
-  cfg.blockDim = dim3(kWarps * 32);
-  cfg.dynamicSmemBytes = bytes;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = p.cluster;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  const cudaError_t e = launch_kernel(kernel, static_cast<unsigned>(groups * p.cluster), kWarps * 32, bytes, stream, p, p.cluster);
   if (e == cudaSuccess) return BSP_OK;
-  (void)cudaGetLastError();
   return fail(BSP_ERR_CUDA, "cache attention: %s", cudaGetErrorString(e));
 }
 

@@ -19,6 +19,7 @@
 #include <cuda_runtime.h>
 
 #include "common.h"
+#include "launch.cuh"
 #include "tile.cuh"
 
 namespace bsp {
@@ -71,6 +72,7 @@ __global__ void __launch_bounds__(kThreads, VEC == 8 && !INTER ? 5 : 4) rotary_k
   // (8192 tokens x 2 x 32 heads of 128: one 51 us, two 58, four 75; with fewer sines the other way round: FP32, 3219 tokens x 15 heads of 80, 9.5 and 8.9 us).
   constexpr int kBatch = VEC == 8 && !INTER ? 1 : 2;
   extern __shared__ float2 cs[];                    // [tokens][pairs]
+  wait_for_earlier_kernels();
   const int tid = threadIdx.x, tokens = 1 << p.log_tokens;
   const int64_t first = static_cast<int64_t>(blockIdx.x) << p.log_tokens, total = static_cast<int64_t>(p.Z) * p.L;
   // A thread keeps one unit of one token, and so its sines, for every head that it takes.
@@ -157,8 +159,7 @@ template <typename T, int VEC, bool INTER> int launch(RotaryParams& p, cudaStrea
   for (p.log_tokens = 0; (2 << p.log_tokens) <= kMaxTokens && total >> p.log_tokens >= 2048 && p.log_units + p.log_tokens < 8; ++p.log_tokens) {}
   const int64_t grid = (total + (1 << p.log_tokens) - 1) >> p.log_tokens;
   if (grid > INT32_MAX) return fail(BSP_ERR_UNSUPPORTED, "rotary: too many tokens (%lld)", (long long)total);
-  rotary_kernel<T, VEC, INTER><<<static_cast<unsigned>(grid), kThreads, sizeof(float2) * p.pairs << p.log_tokens, stream>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const cudaError_t e = launch_kernel(rotary_kernel<T, VEC, INTER>, static_cast<unsigned>(grid), kThreads, sizeof(float2) * p.pairs << p.log_tokens, stream, p);
   return e == cudaSuccess ? BSP_OK : fail(BSP_ERR_CUDA, "rotary: %s", cudaGetErrorString(e));
 }
 
