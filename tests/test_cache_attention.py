@@ -277,6 +277,32 @@ def test_scales_of_either_sign_and_powers_of_two(dtype, T):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('size', [2.0 ** 100, 2.0 ** 124, 2.0 ** -95])
+def test_the_ends_of_bf16(D, size):
+    lengths, H, L = ints(90), 2, 90
+    cache, pages, zero = Guarded(3, H, D, page=32), table(1, 3, 3), ints(0)
+    k, v = tokens(1, H, L, D, torch.bfloat16), (tokens(1, H, L, D, torch.bfloat16, 1).clamp(-7, 7) * size).to(torch.bfloat16)
+    cache.write(k, v, pages, zero)
+    kk, vv = cache.read(pages, zero, L, dtype=torch.float32)
+    layout, there = layouts.dense(1, 3), torch.ones(1, L, dtype=torch.bool)
+    for G in (1, 4, 8):
+        q = queries(1, G * H, 1, D, torch.bfloat16)
+        got = SparseSelfAttention(layout=layout, block=32).decode(q, cache, pages, lengths)
+        assert_decoded(got, q, kk, vv, there, lengths, layout, 32, D ** -0.5)
+
+
+@pytest.mark.gpu
+def test_a_layout_without_blocks():
+    cache, pages, _, _ = filled(1, 2, 40, 64, 16, torch.float16, ints(40))
+    q = queries(1, 2, 1, 64, torch.float16)
+    layout = torch.zeros((2, 3, 3), dtype=torch.int64)
+    assert not bool(SparseSelfAttention(layout=layout, block=16).decode(q, cache, pages, ints(40)).any())
+    with pytest.raises(ValueError):
+        SparseSelfAttention(layout=layout[:1, :0, :0], block=16).decode(q, cache, pages, ints(40))
+
+
+@pytest.mark.gpu
 def test_pages_shared_by_sequences():
     """One prompt's pages in every sequence's table (a row expanded over the batch), read only."""
     H, L, D = 2, 100, 64

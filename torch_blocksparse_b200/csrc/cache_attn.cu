@@ -98,7 +98,7 @@ __device__ __forceinline__ uint32_t pack_half(float lo, float hi) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ float exact_exp2(int e) { return __int_as_float((e + 127) << 23); }   // -126 <= e <= 127
-__device__ __forceinline__ int exponent_of(float x) { return max(-100, min(100, static_cast<int>(__float_as_uint(x) >> 23) - 127)); }
+__device__ __forceinline__ int exponent_of(float x, int most) { return max(-100, min(most, static_cast<int>(__float_as_uint(x) >> 23) - 127)); }
 // One of a pair of bf16 as a float, and times another (exact: 16 significant bits).  Both on the FMA pipe in one instruction:
 // a shift or mask takes the integer pipe two cycles, and that pipe is what the kernel runs out of.
 __device__ __forceinline__ float bf16_at(uint32_t pair, int i) {
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
     // |q| < 2^(e + 1); q * 2^(13 - e) < 2^14, and a sixteenth of it in the odd quarters
-    const int e = exponent_of(amax);
+    const int e = exponent_of(amax, 119);
     const float sign = p.scale_log2e > 0.f ? 1.f : p.scale_log2e < 0.f ? -1.f : p.scale_log2e;   // (scores come out scaled by > 0)
     const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 256.f, 0x1p-100f);           // 2^21 * 2^(e - 13)
 #pragma unroll
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         for (int d = GC > 1 ? 4 : 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
         ratio[k] = 1.f;
         if (t > (k % 2 ? __high2float(ceiling[k / 2]) : __low2float(ceiling[k / 2]))) {
-          const int e = exponent_of(t);            // the largest scale becomes 2^7 .. 2^8 in P
+          const int e = exponent_of(t, 122);       // the largest scale becomes 2^7 .. 2^8 in P
           const float b = exact_exp2(7 - e), old = bf16_at(boost[k / 2], k % 2);
           ratio[k] = old > 0.f ? b / old : 0.f;
           boost[k / 2] = k % 2 ? (boost[k / 2] & 0xffffu) | __float_as_uint(b) : (boost[k / 2] & 0xffff0000u) | __float_as_uint(b) >> 16;
@@ -508,22 +508,9 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   cp_async_wait<0>();
   __syncwarp();
 
-  // ---- join: the warp's sums into its ring, then all warps', then all CTAs' of the cluster
+  // ---- join: the warp's averages into its ring, then all warps', then all CTAs' of the cluster, each with its share of the weight
+  // (sums of values near the end of bf16's range would leave a float's)
   float* own = reinterpret_cast<float*>(ring);     // [queries][D]
-#pragma unroll
-  for (int k = 0; k < NG; ++k) {
-    if (GC == 4 && k / 2 != my_word) continue;
-    const float b = bf16_at(boost[GC == 4 ? 0 : k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
-#pragma unroll
-    for (int i = 0; i < QL; ++i)
-      if (my_query + i < nq)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {              // channel g + 8 j of the group
-          const int column = GC > 1 ? k % 2 : i;
-          own[(my_query + i) * D + k * 32 + g + 8 * j] =
-              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 1.f : 16.f) - eights[k / GC][column]) * 0x1p17f * back;
-        }
-  }
 #pragma unroll
   for (int i = 0; i < QL; ++i) {
 #pragma unroll
@@ -533,30 +520,47 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       part_l[warp][my_query + i] = l[i];
     }
   }
+#pragma unroll
+  for (int k = 0; k < NG; ++k) {
+    if (GC == 4 && k / 2 != my_word) continue;
+    const float b = bf16_at(boost[GC == 4 ? 0 : k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
+#pragma unroll
+    for (int i = 0; i < QL; ++i)
+      if (my_query + i < nq) {
+        const int column = GC > 1 ? k % 2 : i;
+        const float each = l[i] == 0.f ? 0.f : 0x1p17f / l[i];
+#pragma unroll
+        for (int j = 0; j < 4; ++j)                // channel g + 8 j of the group
+          own[(my_query + i) * D + k * 32 + g + 8 * j] =
+              (acc[2 * k + j / 2][column + j % 2 * 2] * (j / 2 ? 1.f : 16.f) - eights[k / GC][column]) * each * back;
+      }
+  }
   __syncthreads();
   T* o = static_cast<T*>(p.o) + z * p.o_sz;
-  auto store = [&](int r, int d, float sum, float weight) {
+  auto store = [&](int r, int d, float value) {
     const int q = r0 + r, t = p.T == 1 ? 0 : q / p.G;
-    o[(hk * p.G + q - t * p.G) * p.o_sh + t * p.o_st + d] = cvt_out<T>(weight > 0.f || weight != weight ? sum / weight : 0.f);
+    o[(hk * p.G + q - t * p.G) * p.o_sh + t * p.o_st + d] = cvt_out<T>(value);
   };
-  // Where there are more CTAs, each sends every one of them the part of the sums that it stores in the end: rank v
+  // Where there are more CTAs, each sends every one of them the part of its averages that it stores in the end: rank v
   // has v * share .. v * share + share - 1.
   const int share = (nq * D + p.cluster - 1) / p.cluster;
   cg::cluster_group cluster = cg::this_cluster();
   if (p.cluster > 1) asm volatile("barrier.cluster.wait.aligned;\n");
   for (int at = threadIdx.x; at < nq * D; at += kWarps * 32) {
     const int r = at / D;
-    float top = kNothing, sum = 0.f, weight = 0.f;
+    float top = kNothing, sum = 0.f, weight = 0.f, share_of[kWarps];
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) top = fmaxf(top, part_m[v][r]);
 #pragma unroll
     for (int v = 0; v < kWarps; ++v) {
-      const float f = fast_exp2(part_m[v][r] - top);
-      weight += part_l[v][r] * f;
-      sum += reinterpret_cast<const float*>(smem + v * (kStages * STAGE))[at] * f;
+      share_of[v] = part_l[v][r] * fast_exp2(part_m[v][r] - top);
+      weight += share_of[v];
     }
+    const float each = weight == 0.f ? 0.f : 1.f / weight;
+#pragma unroll
+    for (int v = 0; v < kWarps; ++v) sum += reinterpret_cast<const float*>(smem + v * (kStages * STAGE))[at] * (share_of[v] * each);
     if (p.cluster == 1) {
-      store(r, at % D, sum, weight);
+      store(r, at % D, sum);
       continue;
     }
     const int to = at / share;
@@ -570,18 +574,21 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
   cluster.sync();
   for (int i = threadIdx.x; i < share && rank * share + i < nq * D; i += kWarps * 32) {
     const int at = rank * share + i, r = at / D;
-    float top = kNothing, sum = 0.f, weight = 0.f;
+    float top = kNothing, sum = 0.f, weight = 0.f, share_of[kMaxCluster];
 #pragma unroll
     for (int v = 0; v < kMaxCluster; ++v)
       if (v < p.cluster) top = fmaxf(top, inbox_m[v][r]);
 #pragma unroll
     for (int v = 0; v < kMaxCluster; ++v)
       if (v < p.cluster) {
-        const float f = fast_exp2(inbox_m[v][r] - top);
-        weight += inbox_l[v][r] * f;
-        sum += inbox[v * share + i] * f;
+        share_of[v] = inbox_l[v][r] * fast_exp2(inbox_m[v][r] - top);
+        weight += share_of[v];
       }
-    store(r, at % D, sum, weight);
+    const float each = weight == 0.f ? 0.f : 1.f / weight;
+#pragma unroll
+    for (int v = 0; v < kMaxCluster; ++v)
+      if (v < p.cluster) sum += inbox[v * share + i] * (share_of[v] * each);
+    store(r, at % D, sum);
   }
 }
 
@@ -652,7 +659,7 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   // one 6.4; 8 x 16 heads, 36 blocks: 4 CTAs 9.9 us, one 16.3, 8 CTAs, which do not fit, 14.6), and a granule of an average row
   // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys, eight
   // queries each: 107 us, one at a time 119); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 11.3 us, one at a time 9.9).
-  const int64_t granules = (static_cast<int64_t>(mt.nnz) / (static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
+  const int64_t granules = (static_cast<int64_t>(mt.nnz) / std::max<int64_t>(1, static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
   p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * 148 / groups, granules / kWarps})));
   const bool many = granules > 16 * kWarps * p.cluster;
   if (Z > INT32_MAX / Hk / p.tiles / p.cluster) return fail(BSP_ERR_UNSUPPORTED, "cache attention: too many queries");
