@@ -21,10 +21,13 @@
 //
 // Numbers.  q is scaled by a power of two to the top of fp16's range and so keeps every bit of either type down to
 // 2^-24 of the row's largest.  Scores, sums, maxima and accumulators are floats.  P is rounded to half:
-// 2^-12 relative, an eighth of bf16's half step; for fp16 results a second product adds what the rounding
-// cut off (SPLIT).  The largest scale seen so far of each group fixes a power of two that keeps P in
-// half's range; maxima and those powers are renewed only when exceeded by 2^4 and 2^3 (exact, since
-// everything is relative to them), so that a granule usually costs one vote.
+// 2^-11 relative, an eighth of bf16's half step; for fp16 results a second product adds what the rounding
+// cut off (SPLIT).  A power of two for each query and group keeps P in half's range.  It follows the largest p * s, not
+// the largest s (a large value that a query gives no weight would push the others' P into half's subnormal range), so what is lost
+// there is at most 2^-32 of the largest product of a weight and a scale for each key.  A warp usually finds with one vote that
+// it need not look closer: no score is 2^4 above the maximum, and no scale so large that its P could pass 2^15.  Where one is, or some
+// queries do not see all tokens, every P is checked and the powers are lowered where one is above 2^8 (exact, since everything is
+// relative to them); a new maximum, which makes all weights smaller, raises them.
 //
 // Work: a CTA's warps, times the CTAs of a cluster, take the granules of one (sequence, head, eight
 // queries) in turn, each through a ring of its own (cp.async, no barriers), and join their sums
@@ -60,6 +63,8 @@ constexpr int kMaxCluster = 8;
 constexpr float kNothing = -3e38f; // the maximum of no scores
 constexpr float kSlack = 4.f;      // p <= 2^4
 constexpr uint32_t kEights = 0x04000400u;        // halves 2^-14: 8 as a code in a high field
+constexpr uint32_t kSixteenth = 0x3d803d80u;     // a pair of bf16
+constexpr int kHighest = 234, kLowest = 12;   // biased exponents of the powers of two on P: 2^107, 2^-115
 constexpr int kNone = 0x7ffffff0;  // the token of a granule that is not there: nobody sees it
 
 struct AttnParams {
@@ -107,11 +112,18 @@ __device__ __forceinline__ float bf16_at(uint32_t pair, int i) {
   else asm("{.reg .b16 l, h; mov.b32 {l, h}, %1; add.rn.f32.bf16 %0, l, 0f00000000;}" : "=f"(x) : "r"(pair));
   return x;
 }
-__device__ __forceinline__ float bf16_product(uint32_t pair, uint32_t other, int i) {
+__device__ __forceinline__ float bf16_product(uint32_t pair, int i, uint32_t other, int j) {
   float x;
-  if (i) asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, h, n, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
+  if (i && j) asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, h, n, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
+  else if (i) asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, h, m, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
+  else if (j) asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, l, n, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
   else asm("{.reg .b16 l, h, m, n; mov.b32 {l, h}, %1; mov.b32 {m, n}, %2; fma.rn.f32.bf16 %0, l, m, 0f00000000;}" : "=f"(x) : "r"(pair), "r"(other));
   return x;
+}
+// The biased exponents of a pair of powers of two in bf16.
+__device__ __forceinline__ int exponent_at(uint32_t pair, int i) { return pair >> (16 * i + 7) & 255; }
+__device__ __forceinline__ void set_exponent(uint32_t& pair, int i, int e) {
+  pair = (pair & (i ? 0x0000ffffu : 0xffff0000u)) | static_cast<uint32_t>(e) << (16 * i + 7);
 }
 __device__ __forceinline__ __nv_bfloat162 as_bf162(uint32_t x) { return *reinterpret_cast<const __nv_bfloat162*>(&x); }
 
@@ -286,13 +298,31 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     m[i] = limit_m[i] = -INFINITY;
     neg_m[i] = l[i] = 0.f;
   }
-  uint32_t boost[SW];                              // powers of two on P, pairs of bf16
-  __nv_bfloat162 ceiling[SW];                      // scales of V above which new ones are due
+  // Powers of two on P, pairs of bf16: of a set's two groups, or (GC = 1) of a group's two queries.  Scales of V above which
+  // P could pass 2^15 while p <= 2^4, by group; none for a query that has seen nothing, whose P are zeros.
+  uint32_t boost[SETS];
+  __nv_bfloat162 ceiling[SW];
 #pragma unroll
-  for (int k = 0; k < SW; ++k) {
-    boost[k] = 0;
-    ceiling[k] = as_bf162(0);
-  }
+  for (int k = 0; k < SETS; ++k) boost[k] = 0x3f803f80u;
+#pragma unroll
+  for (int k = 0; k < SW; ++k) ceiling[k] = as_bf162(0x7f807f80u);
+  auto renew_ceilings = [&] {
+    auto most = [&](int k, int j) { return m[GC == 1 ? j : 0] == -INFINITY ? 0x7f80u : static_cast<uint32_t>(265 - exponent_at(boost[k], j)) << 7; };
+#pragma unroll
+    for (int k = 0; k < SW; ++k) {
+      if constexpr (GC == 1) ceiling[k] = as_bf162(min(most(2 * k, 0), most(2 * k, 1)) | min(most(2 * k + 1, 0), most(2 * k + 1, 1)) << 16);
+      else ceiling[k] = as_bf162(most(k, 0) | most(k, 1) << 16);
+    }
+  };
+  // Sums of the k-th set by columns, times f
+  auto scale_sums = [&](int k, float f0, float f1) {
+#pragma unroll
+    for (int n = 2 * GC * k; n < 2 * GC * (k + 1); ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[n][i] *= i % 2 ? f1 : f0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) eights[k][i] *= i % 2 ? f1 : f0;
+  };
 
   // NP granules at a time: what is done once for them (waiting, voting, branching) is a good part of the work,
   // and they hide each other's latencies
@@ -381,7 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       }
     }
 
-    // renew the maxima and powers of two where they are exceeded
+    // new maxima where they are exceeded; whether every P is to be checked
     float top[QL];
     __nv_bfloat162 scale_top[SW];
 #pragma unroll
@@ -397,49 +427,34 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     uint32_t over = 0;
 #pragma unroll
     for (int k = 0; k < SW; ++k) over |= __hgt2_mask(scale_top[k], ceiling[k]);
-    bool due = over;
+    bool due = false;
 #pragma unroll
     for (int i = 0; i < QL; ++i) due = due || top[i] > limit_m[i];
-    if (__any_sync(~0u, due)) {
-      float f[QL], ratio[2 * SW];
+    bool careful = masked, fallen = false;
+    float fall[QL];                                // of all weights so far, as a power of two
 #pragma unroll
-      for (int i = 0; i < QL; ++i) {
-        float t = top[i];
+    for (int i = 0; i < QL; ++i) fall[i] = 0.f;
+    if (__any_sync(~0u, due || over)) {
+      careful = true;
+      fallen = __any_sync(~0u, due);
+      if (fallen) {
 #pragma unroll
-        for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-        f[i] = 1.f;
-        if (t > m[i]) {
-          f[i] = fast_exp2((m[i] - t) * unscale[i]);
-          m[i] = t;
-          neg_m[i] = -t * unscale[i];
-          limit_m[i] = t + kSlack / unscale[i];
-        }
-        l[i] *= f[i];
-      }
+        for (int i = 0; i < QL; ++i) {
+          float t = top[i];
 #pragma unroll
-      for (int k = 0; k < 2 * SW; ++k) {
-        float t = k % 2 ? __high2float(scale_top[k / 2]) : __low2float(scale_top[k / 2]);
-        // (lanes with the same columns; with GC = 1 every lane has all groups, of tokens that one of its queries sees)
-#pragma unroll
-        for (int d = GC > 1 ? 4 : 1; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
-        ratio[k] = 1.f;
-        if (t > (k % 2 ? __high2float(ceiling[k / 2]) : __low2float(ceiling[k / 2]))) {
-          const int e = exponent_of(t, 122);       // the largest scale becomes 2^7 .. 2^8 in P
-          const float b = exact_exp2(7 - e), old = bf16_at(boost[k / 2], k % 2);
-          ratio[k] = old > 0.f ? b / old : 0.f;
-          boost[k / 2] = k % 2 ? (boost[k / 2] & 0xffffu) | __float_as_uint(b) : (boost[k / 2] & 0xffff0000u) | __float_as_uint(b) >> 16;
-          const __nv_bfloat16 c = __float2bfloat16_rn(exact_exp2(e + 4));
-          ceiling[k / 2] = k % 2 ? __halves2bfloat162(__low2bfloat16(ceiling[k / 2]), c) : __halves2bfloat162(c, __high2bfloat16(ceiling[k / 2]));
+          for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+          if (t > m[i]) {
+            fall[i] = (t - m[i]) * unscale[i];
+            m[i] = t;
+            neg_m[i] = -t * unscale[i];
+            limit_m[i] = t + kSlack / unscale[i];
+            l[i] *= fast_exp2(-fall[i]);
+          }
         }
       }
+      if (!masked)
 #pragma unroll
-      for (int n = 0; n < NK; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[n][i] *= f[i % QL] * ratio[GC == 1 ? n / 2 : GC == 2 ? n / 4 * 2 + i % 2 : i % 2];
-#pragma unroll
-      for (int k = 0; k < SETS; ++k)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) eights[k][i] *= f[i % QL] * ratio[GC == 1 ? k : GC == 2 ? 2 * k + i % 2 : i % 2];
+        for (int u = 0; u < NP; ++u) keep[u][0] = keep[u][1] = ~0u;
     }
 
 #pragma unroll
@@ -449,30 +464,62 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         x[u][i] = fast_exp2(fmaf(x[u][i], unscale[i % QL], neg_m[i % QL]));
         l[i % QL] += x[u][i];
       }
-    auto add_values = [&](auto some_unseen) {
+    auto add_values = [&](auto check) {
 #pragma unroll
       for (int u = 0; u < NP; ++u) {
         // P as operands, of the k-th set, and with SPLIT what its rounding cut off
         uint32_t b[SPLIT ? 2 : 1][2];
         auto weights = [&](int k) {
+          float w[2][2];                           // by token half and column
+          if constexpr (check) {
+            // (x * s first: s * boost may leave a float's range where x is small; a sixteenth, for x is up to 2^4)
+            auto part = [&](int v, int i, int j) {
+              return GC > 1 ? x[v][i] * bf16_product(vs[v][i][k], j, kSixteenth, 0) : x[v][2 * i + j] * bf16_product(vs[v][i][k / 2], k % 2, kSixteenth, 0);
+            };
+            auto multiply = [&] {
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                const float by = bf16_at(boost[k], j) * 16.f;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[i][j] = part(u, i, j) * by;
+              }
+            };
+            multiply();
+            if ((u == 0 && fallen) || __any_sync(~0u, fmaxf(fmaxf(w[0][0], w[1][0]), fmaxf(w[0][1], w[1][1])) > 256.f)) {
+              float f[2];
+#pragma unroll
+              for (int j = 0; j < 2; ++j) {
+                float t = 0.f;
+#pragma unroll
+                for (int v = 0; v < NP; ++v) t = fmaxf(t, fmaxf(part(v, 0, j), part(v, 1, j)));
+#pragma unroll
+                for (int d = 4; d < 32; d *= 2) t = fmaxf(t, __shfl_xor_sync(~0u, t, d));
+                // as high as the fall of the weights allows, and the largest P of the step at 2^7 .. 2^8 at most
+                const float by = u ? 0.f : fall[GC == 1 ? j : 0];
+                const int old = exponent_at(boost[k], j), most = by < 126.f ? min(old + static_cast<int>(ceilf(by)), kHighest) : kHighest;
+                const int e = max(kLowest, min(most, 134 - (static_cast<int>(__float_as_uint(t) >> 23) - 127 + 4)));
+                set_exponent(boost[k], j, e);
+                f[j] = by < 126.f && old - e < 127 ? exact_exp2(e - old) * fast_exp2(-by) : 0.f;
+              }
+              scale_sums(k, f[0], f[1]);
+              multiply();
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int j = 0; j < 2; ++j)
+                w[i][j] = GC > 1 ? x[u][i] * bf16_product(vs[u][i][k], j, boost[k], j) : x[u][2 * i + j] * bf16_product(vs[u][i][k / 2], k % 2, boost[k], j);
+          }
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            float w0, w1;
-            if constexpr (GC > 1) {
-              w0 = x[u][i] * bf16_product(vs[u][i][k], boost[k], 0);
-              w1 = x[u][i] * bf16_product(vs[u][i][k], boost[k], 1);
-            } else {
-              const float s = bf16_product(vs[u][i][k / 2], boost[k / 2], k % 2);
-              w0 = x[u][2 * i] * s;
-              w1 = x[u][2 * i + 1] * s;
-            }
-            uint32_t h = pack_half(w0, w1);
-            if constexpr (some_unseen) h &= keep[u][i];   // (0 times a NaN scale of a token that this query does not see)
+            uint32_t h = pack_half(w[i][0], w[i][1]);
+            if constexpr (check) h &= keep[u][i];  // (0 times a NaN scale of a token that this query does not see)
             b[0][i] = transpose8(h);
             if constexpr (SPLIT) {
               const float2 r = __half22float2(*reinterpret_cast<const __half2*>(&h));
-              uint32_t rest = pack_half(w0 - r.x, w1 - r.y);
-              if constexpr (some_unseen) rest &= keep[u][i];
+              uint32_t rest = pack_half(w[i][0] - r.x, w[i][1] - r.y);
+              if constexpr (check) rest &= keep[u][i];
               b[1][i] = transpose8(rest);
             }
           }
@@ -498,8 +545,12 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
         }
       }
     };
-    if (masked) add_values(std::true_type());
-    else add_values(std::false_type());
+    if (careful) {
+      add_values(std::true_type());
+      renew_ceilings();
+    } else {
+      add_values(std::false_type());
+    }
     __syncwarp();                                  // (all lanes are done with the stage)
 #pragma unroll
     for (int u = 0; u < NP; ++u) tokens[u] = ahead[u];
@@ -523,10 +574,10 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
 #pragma unroll
   for (int k = 0; k < NG; ++k) {
     if (GC == 4 && k / 2 != my_word) continue;
-    const float b = bf16_at(boost[GC == 4 ? 0 : k / 2], k % 2), back = b > 0.f ? 1.f / b : 0.f;
 #pragma unroll
     for (int i = 0; i < QL; ++i)
       if (my_query + i < nq) {
+        const float back = 1.f / bf16_at(boost[k / GC], GC > 1 ? k % 2 : i);
         const int column = GC > 1 ? k % 2 : i;
         const float each = l[i] == 0.f ? 0.f : 0x1p17f / l[i];
 #pragma unroll
