@@ -562,7 +562,8 @@ int bsp_cache_read(void* k, void* v, int dtype, int Z, int H, int T, int D,
  * o = softmax(scale * q K^T) V.  q, o [Z, Hq, T, D] (FP16 or BF16, unit stride
  * on D; q's other strides even, its base on 4 bytes); query head h reads head h / (Hq / Hk) of the cache.  meta: metadata
  * of a square layout of 1 or Hk heads.  Queries that see nothing (positions below
- * zero or behind the layout's last row, pages that are none) give zeros.
+ * zero or behind the layout's last row, pages that are none) give zeros; where scale
+ * times a query's largest channel is above 2^119 its result is NaN.
  */
 int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D,
                    int64_t q_sz, int64_t q_sh, int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st,

@@ -116,3 +116,21 @@ def test_most_weight_on_tiny_values_and_scores_that_climb(dtype, D, G):
     q = torch.ones((2, G, 1, D), device='cuda').to(dtype)
     got, kk, vv = decoded(q, k.to(dtype), v.to(dtype), ints(L, L))
     assert_near(got, q, kk, vv, ints(L, L), D ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('G,T', [(1, 1), (4, 1), (8, 1), (1, 5)])
+def test_queries_up_to_the_end_of_bf16(D, G, T):
+    """A power of two between the query and the scale changes no bit, up to the largest exponent; scores beyond a float's range are NaN."""
+    L = 200
+    k, v = tokens(1, 2, L, D, torch.bfloat16).clamp(-2, 2), tokens(1, 2, L, D, torch.bfloat16, 1)
+    q = tokens(1, 2 * G, T, D, torch.bfloat16, 2).clamp(-7.5, 7.5) * 0.125
+    q[..., 3] = 0.875                                   # (every query has the same exponent, so every one reaches the end)
+    want, kk, vv = decoded(q, k, v, ints(L), scale=0.5)
+    assert_near(want, q, kk, vv, ints(L), 0.5)
+    for shift in (100, 119, 122, 125, 127):
+        far = q * 2.0 ** (shift - 20) * 2.0 ** 20
+        assert bool(far.isfinite().all())
+        assert torch.equal(decoded(far, k, v, ints(L), scale=2.0 ** (-1 - min(shift, 120)))[0], decoded(q, k, v, ints(L), scale=2.0 ** (shift - min(shift, 120) - 1))[0])
+    assert bool(decoded(q * 2.0 ** 126, k, v, ints(L), scale=1.0)[0].isnan().all())

@@ -216,7 +216,8 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         the nonzero blocks of its block-row: what forward() gives for that row under a causal
         attn_mask.  The layout is the module's own, [heads of the cache or 1, ...], or its configuration's for
         sequences as long as the page table; rows behind its end see nothing.  Positions below zero
-        (sequences shorter than T) and queries that see nothing give zeros.  scale: head_dim ** -0.5.
+        (sequences shorter than T) and queries that see nothing give zeros.  scale: head_dim ** -0.5;
+        where scale times a query's largest channel is above 2 ** 119 its result is NaN.
 
         One kernel, without workspace, on the current stream of the cache's device; no gradient.  Lengths
         and tables are read on the device, so that a captured call can be replayed as sequences grow (the

@@ -260,10 +260,11 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
       for (int i = 0; i < 2; ++i) amax = fmaxf(amax, fmaxf(fabsf(pair_at(n, i).x), fabsf(pair_at(n, i).y)));
     amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(~0u, amax, 2));
-    // |q| < 2^(e + 1); q * 2^(13 - e) < 2^14, and a sixteenth of it in the odd quarters
-    const int e = exponent_of(amax, 119);
+    // |q| < 2^(e + 1); q * 2^(13 - e) < 2^14, and a sixteenth of it in the odd quarters.  (Where scale * 2^e is above 2^119 the
+    // factor that takes this back, 2^8 times that, is infinite, and so the query's scores are no numbers.)
+    const int e = exponent_of(amax, 127);
     const float sign = p.scale_log2e > 0.f ? 1.f : p.scale_log2e < 0.f ? -1.f : p.scale_log2e;   // (scores come out scaled by > 0)
-    const float down = fmaxf(fabsf(p.scale_log2e) * exact_exp2(e) * 256.f, 0x1p-100f);           // 2^21 * 2^(e - 13)
+    const float down = fmaxf(fabsf(p.scale_log2e) * 256.f * exact_exp2(e), 0x1p-100f);           // 2^21 * 2^(e - 13)
 #pragma unroll
     for (int i = 0; i < QL; ++i) unscale[i] = __shfl_sync(~0u, down, (GC == 1 ? my_query + i : my_query * GC) * 4);
     const float up = exact_exp2(13 - e) * sign;
