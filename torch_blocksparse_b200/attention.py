@@ -73,6 +73,18 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         self._causal_cache = dict()
         self.causal_checks = 0            # comparisons of a mask against the causal one made so far
 
+    def __setattr__(self, name, value):
+        # The tables of a layout go with it, before the operations made of them do (so that no call puts an operation of the
+        # old tables into the new cache), and a configuration brings its block.  (An explicit layout that no longer fits
+        # a changed block keeps its tables, which every call then refuses.)
+        known = self.__dict__
+        if 'ops' in known and (name in ('layout', 'sparsity_config') or (name == 'block' and known.get('layout') is None)):
+            super(_lib.WithOps, self).__setattr__(name, value)
+            self.ops, self.tiles = dict(), dict()
+            if name == 'sparsity_config' and known.get('layout') is None:
+                self.block = value.block
+        super().__setattr__(name, value)
+
     def get_layout(self, H, L):
         """The [H, L/block, L/block] layout used for H heads and sequence length L."""
         block = self.block
@@ -91,21 +103,24 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
     def get_ops(self, H, L):
         """(sdd_nt, dsd_nn, softmax) for H heads of length L, built once
         (deepspeedsparseselfattention.py:67-106)."""
-        key = (H, L)
-        if key not in self.ops:
-            layout = self.get_layout(H, L)
-            sdd_nt = MatMul(layout, self.block, 'sdd', trans_a=False, trans_b=True)
-            dsd_nn = MatMul(layout, self.block, 'dsd', trans_a=False, trans_b=False)
+        key, ops, tiles = (H, L), self.ops, self.tiles      # (before the attributes: see __setattr__)
+        found = ops.get(key)
+        if found is None:
+            layout, block = self.get_layout(H, L), self.block
+            sdd_nt = MatMul(layout, block, 'sdd', trans_a=False, trans_b=True)
+            dsd_nn = MatMul(layout, block, 'dsd', trans_a=False, trans_b=False)
             dsd_nn._meta = sdd_nt.meta            # one metadata buffer per layout
-            self.ops[key] = (sdd_nt, dsd_nn, Softmax(layout, self.block))
-            self.tiles[key] = tables.build_attn_tiles(layout, self.block) if self.fused else None
-        return self.ops[key]
+            found = (sdd_nt, dsd_nn, Softmax(layout, block))
+            tiles[key] = sdd_nt.attn_tiles = tables.build_attn_tiles(layout, block) if self.fused else None
+            ops[key] = found
+        return found
 
     def _attn_op(self, query, H, L):
         """The fused attention with this module's tables on the device of `query`."""
         ops = self._attn
         sdd_nt, _, _ = self.get_ops(H, L)
-        op = fused.Attention(sdd_nt.meta, self.tiles[(H, L)], self.block, query.device)
+        tiles = sdd_nt.attn_tiles if hasattr(sdd_nt, 'attn_tiles') else self.tiles[(H, L)]   # (in modules saved earlier)
+        op = fused.Attention(sdd_nt.meta, tiles, self.block, query.device)
         ops[(H, L, query.get_device())] = op
         return op
 
