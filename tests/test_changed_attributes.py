@@ -61,3 +61,44 @@ def test_forward_and_decode_follow_a_changed_layout(fused):
     fresh = SparseSelfAttention(SparsityConfig(block=32, stride=32), fused=fused)
     assert torch.equal(attn(q, k, v), fresh(q, k, v))
     assert torch.equal(attn.decode(q[:, :, -1:], cache, pages, ints(L)), fresh.decode(q[:, :, -1:], cache, pages, ints(L)))
+
+
+@pytest.mark.gpu
+def test_operations_built_while_an_attribute_changes_are_not_kept():
+    class ChangingCache(KVCache):
+        armed = False
+
+        @property
+        def head_dim(self):
+            if self.armed:                             # (as another thread would, while the operation is built)
+                self.armed = False
+                self.data = other
+            return 64
+
+        @head_dim.setter
+        def head_dim(self, value):
+            pass
+
+    cache = ChangingCache(2, 1, 64, page=16)
+    other = torch.zeros_like(cache.data)
+    cache.armed = True
+    cache._op()
+    x = tokens(1, 1, 16, 64, torch.float16)
+    cache.write(x, x, table(1, 2, 2), ints(0))
+    assert bool(other.any())
+
+    class Changing(SparseSelfAttention):
+        def _decode_op(self, ops, key, cache, device):
+            op = super()._decode_op(ops, key, cache, device)
+            if self.layout is first:
+                self.layout = second
+                ops[key] = op                          # (as a thread that was interrupted before it stored the operation)
+            return op
+
+    first, second = layouts.dense(1, 2), layouts.causal_band(1, 2, 1)
+    attn, cache, pages = Changing(layout=first, block=16), KVCache(2, 1, 64, page=16), table(1, 2, 2)
+    k = tokens(1, 1, 32, 64, torch.float16)
+    cache.write(k, k, pages, ints(0))
+    attn.decode(k[:, :, -1:], cache, pages, ints(32))
+    want = SparseSelfAttention(layout=second, block=16).decode(k[:, :, -1:], cache, pages, ints(32))
+    assert torch.equal(attn.decode(k[:, :, -1:], cache, pages, ints(32)), want)

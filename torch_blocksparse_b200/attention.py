@@ -238,18 +238,19 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         and tables are read on the device, so that a captured call can be replayed as sequences grow (the
         first call for a layout uploads its tables: not inside a capture)."""
         cache_op = cache._op()
+        ops = self._attn
         key = (cache_op.heads, query.get_device(), None if self.layout is not None else pages.size(-1) * cache.page, 'decode')
-        op = self._attn.get(key) or self._decode_op(key, cache, query.device)
+        op = ops.get(key) or self._decode_op(ops, key, cache, query.device)
         return op(query, cache_op, pages, lengths, scale)
 
-    def _decode_op(self, key, cache, device):
+    def _decode_op(self, ops, key, cache, device):
         layout = self.layout
         if layout is None:
             layout = self.get_layout(cache.num_heads, -(-key[2] // self.block) * self.block)
         elif layout.size(0) not in (1, cache.num_heads):
             raise ValueError(f'a layout of {layout.size(0)} heads does not fit a cache of {cache.num_heads}')
         meta = tables.build_meta(layout)
-        op = self._attn[key] = _lib.ops().CacheAttentionOp(meta.hdr, meta.on(device), self.block)
+        op = ops[key] = _lib.ops().CacheAttentionOp(meta.hdr, meta.on(device), self.block)
         return op
 
 

@@ -56,13 +56,14 @@ class KVCache(_lib.WithOps):
     def _op(self):
         if recording() is not None:
             raise RuntimeError('a KVCache changes between calls, which torch.jit.trace cannot replay')
-        op = self._ops.get('op')
+        ops = self._ops                      # (before the attributes: see WithOps)
+        op = ops.get('op')
         if op is None:
             d = self.data
             if d.dtype != torch.uint8 or not d.is_cuda or d.dim() != 3 or not d.is_contiguous() or \
                     d.size(2) != _lib.lib().bsp_cache_page_bytes(self.page, self.head_dim):
                 raise ValueError('data must be a contiguous uint8 CUDA tensor [pages, heads, bytes of a page]')
-            op = self._ops['op'] = _lib.ops().CacheOp(d, self.page, self.head_dim)
+            op = ops['op'] = _lib.ops().CacheOp(d, self.page, self.head_dim)
         return op
 
     def write(self, key, value, pages, start, count=None):
