@@ -429,6 +429,26 @@ def test_a_configuration_and_changed_attributes():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('config', [dict(), dict(stride=128, numverts=3), dict(attention='bidirectional', stride=32), dict(mode='dense')])
+@pytest.mark.parametrize('page', [16, 32])
+def test_a_configuration_and_a_table_that_grows_page_by_page(config, page):
+    """Widths that fill no window of the layout among them; lengths behind the table see nothing."""
+    H, D, most = 2, 64, 12
+    config = SparsityConfig(block=16, **config)
+    attn, windows = SparseSelfAttention(config), -(-most * page // config.stride)
+    layout = attn.get_layout(H, windows * config.stride)
+    cache, pages, k, v = filled(3, H, most * page, D, page, torch.float16, ints(*[most * page] * 3))
+    q, there = queries(3, H, 2, D, torch.float16), torch.ones(3, most * page, dtype=torch.bool)
+    for slots in range(1, most + 1):
+        n = slots * page
+        lengths = ints(n, max(0, n - 7), n + 50)
+        got = attn.decode(q, cache, pages[:, :slots], lengths)
+        assert_decoded(got, q, k[:, :, :n], v[:, :, :n], there[:, :n], lengths, layout[:, :n // 16, :n // 16], 16, D ** -0.5)
+        assert not bool(got[2].any())
+    assert not bool(attn.decode(q, cache, pages[:, :0], lengths).any())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('kind', ['fixed', 'band'])
 def test_rotated_written_and_decoded_as_the_whole_sequence(kind):
     """A prompt and then token after token, against forward() on the whole sequence with the cache's values."""

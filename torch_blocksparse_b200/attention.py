@@ -246,7 +246,9 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
     def _decode_op(self, ops, key, cache, device):
         layout = self.layout
         if layout is None:
-            layout = self.get_layout(cache.num_heads, -(-key[2] // self.block) * self.block)
+            rows = max(1, -(-key[2] // self.block))
+            window = max(1, self.sparsity_config.stride // self.block)       # (layouts are made of whole windows)
+            layout = self.get_layout(cache.num_heads, -(-rows // window) * window * self.block)[:, :rows, :rows]
         elif layout.size(0) not in (1, cache.num_heads):
             raise ValueError(f'a layout of {layout.size(0)} heads does not fit a cache of {cache.num_heads}')
         meta = tables.build_meta(layout)
