@@ -564,12 +564,19 @@ int bsp_cache_read(void* k, void* v, int dtype, int Z, int H, int T, int D,
  * of a square layout of 1 or Hk heads.  Queries that see nothing (positions below
  * zero or behind the layout's last row, pages that are none) give zeros; where scale
  * times a query's largest channel is above 2^119 its result is NaN.
+ * bsp_cache_attn_rows: the same with the first `rows` rows of the layout alone (fewer
+ * than it has: one layout serves sequences of growing capacity).
  */
 int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D,
                    int64_t q_sz, int64_t q_sh, int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st,
                    const void* data, int num_pages, int page, const int32_t* pages, int64_t pages_sz, int slots,
                    const int32_t* lengths, int block, const int32_t* meta_hdr, const int32_t* meta,
                    float scale, void* stream);
+int bsp_cache_attn_rows(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D,
+                        int64_t q_sz, int64_t q_sh, int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st,
+                        const void* data, int num_pages, int page, const int32_t* pages, int64_t pages_sz, int slots,
+                        const int32_t* lengths, int block, const int32_t* meta_hdr, const int32_t* meta,
+                        int rows, float scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -449,6 +449,20 @@ def test_a_configuration_and_a_table_that_grows_page_by_page(config, page):
 
 
 @pytest.mark.gpu
+def test_a_growing_table_builds_few_layouts():
+    attn = SparseSelfAttention(SparsityConfig(block=16, stride=32))
+    cache, q = KVCache(4, 1, 64, page=16), queries(1, 1, 1, 64, torch.float16)
+    x = tokens(1, 1, 64, 64, torch.float16)
+    cache.write(x, x, ints(0, 1, 2, 3)[None], ints(0))
+    pages = ints(0, 1, 2, 3, *[-1] * 396)[None]
+    before, want = tables.CACHE_STATS['misses'], attn.decode(q, cache, pages[:, :4], ints(60))
+    for slots in range(4, 401):
+        assert torch.equal(attn.decode(q, cache, pages[:, :slots], ints(60)), want), slots
+        assert not bool(attn.decode(q, cache, pages[:, :slots], ints(16 * slots + 1)).any())    # behind the table
+    assert tables.CACHE_STATS['misses'] - before <= 8 * 8
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('kind', ['fixed', 'band'])
 def test_rotated_written_and_decoded_as_the_whole_sequence(kind):
     """A prompt and then token after token, against forward() on the whole sequence with the cache's values."""
@@ -555,3 +569,10 @@ def test_bad_calls():
         SparseSelfAttention(layout=layouts.dense(3, 3), block=16).decode(q, cache, pages, lengths)
     with pytest.raises(RuntimeError, match='trace'):
         torch.jit.trace(lambda x: attn.decode(x, cache, pages, lengths), (q,), check_trace=False)
+
+
+def test_the_library_rejects_rows_that_a_layout_does_not_have():
+    L, m = _lib.lib(), tables.build_meta(torch.ones((2, 3, 3), dtype=torch.long))
+    for rows in (-1, 4):
+        assert L.bsp_cache_attn_rows(16, 16, _lib.F16, 1, 4, 2, 1, 64, 64, 64, 64, 64, 64, 64, 16, 1, 64, 16, 1, 1, 16, 16, m.hdr.data_ptr(), 16,
+                                     rows, 1.0, None) == _lib.ERR_INVALID and b'rows' in L.bsp_last_error()

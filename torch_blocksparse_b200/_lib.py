@@ -76,6 +76,8 @@ _SIGNATURES = {
     'bsp_cache_read': (c_int, [c_void_p, c_void_p] + [c_int] * 5 + [c_int64] * 6 + _CACHE + [c_void_p] * 3),
     'bsp_cache_attn': (c_int, [c_void_p, c_void_p] + [c_int] * 6 + [c_int64] * 6 + _CACHE
                        + [c_void_p, c_int, c_void_p, c_void_p, c_float, c_void_p]),
+    'bsp_cache_attn_rows': (c_int, [c_void_p, c_void_p] + [c_int] * 6 + [c_int64] * 6 + _CACHE
+                            + [c_void_p, c_int, c_void_p, c_void_p, c_int, c_float, c_void_p]),
 }
 
 

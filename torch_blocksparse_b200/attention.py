@@ -246,13 +246,20 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
     def _decode_op(self, ops, key, cache, device):
         layout = self.layout
         if layout is None:
-            rows = max(1, -(-key[2] // self.block))
-            window = max(1, self.sparsity_config.stride // self.block)       # (layouts are made of whole windows)
-            layout = self.get_layout(cache.num_heads, -(-rows // window) * window * self.block)[:, :rows, :rows]
-        elif layout.size(0) not in (1, cache.num_heads):
-            raise ValueError(f'a layout of {layout.size(0)} heads does not fit a cache of {cache.num_heads}')
-        meta = tables.build_meta(layout)
-        op = ops[key] = _lib.ops().CacheAttentionOp(meta.hdr, meta.on(device), self.block)
+            # Layouts are made of whole windows; about 8 sizes between one power of two and the next serve tables of any
+            # width (a table that grows page by page builds one now and then), each by its first rows.
+            rows, block = max(1, -(-key[2] // self.block)), self.block
+            window = max(1, self.sparsity_config.stride // block)
+            step = window * max(1, (1 << rows.bit_length() >> 4) // window)
+            size = -(-rows // step) * step
+            meta = ops.get((*key[:2], size, 'rows'))
+            if meta is None:
+                meta = ops[(*key[:2], size, 'rows')] = tables.build_meta(self.get_layout(cache.num_heads, size * block))
+        else:
+            if layout.size(0) not in (1, cache.num_heads):
+                raise ValueError(f'a layout of {layout.size(0)} heads does not fit a cache of {cache.num_heads}')
+            rows, block, meta = layout.size(1), self.block, tables.build_meta(layout)
+        op = ops[key] = _lib.ops().CacheAttentionOp(meta.hdr, meta.on(device), block, rows)
         return op
 
 

@@ -75,7 +75,7 @@ struct AttnParams {
   CachePages pages;
   const int32_t* lengths;
   const int32_t *row_ptr, *blk_col;
-  int layout_heads, layout_rows, block_shift;   // block_shift: log2(granules of a block)
+  int layout_heads, layout_rows, rows, block_shift;   // rows: those that count; block_shift: log2(granules of a block)
   int T, G, tiles, cluster;                     // G: query heads of a cache head; tiles of 8 queries
   float scale_log2e;
 };
@@ -181,7 +181,7 @@ __global__ void __launch_bounds__(kWarps * 32, kCtas) cache_attn_kernel(const __
     for (int s = 0; s < 2; ++s) {
 #pragma unroll
       for (int i = 0; i < QL; ++i) limit[s][i] = s ? -1 : last_pos;
-      if (last_pos < 0 || row[s] >= p.layout_rows || (s && row[1] == row[0])) continue;
+      if (last_pos < 0 || row[s] >= p.rows || (s && row[1] == row[0])) continue;
       begin[s] = row_ptr[row[s]];
       granules[s] = (row_ptr[row[s] + 1] - begin[s]) << p.block_shift;
       last[s] = static_cast<int>(min(static_cast<int64_t>(last_pos), (static_cast<int64_t>(row[s] + 1) << block_log2) - 1));
@@ -667,10 +667,10 @@ template <typename T, int D> int pick(const AttnParams& p, int64_t groups, int q
 }  // namespace
 }  // namespace bsp
 
-extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D, int64_t q_sz, int64_t q_sh,
-                              int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st, const void* data, int num_pages, int page,
-                              const int32_t* pages, int64_t pages_sz, int slots, const int32_t* lengths, int block,
-                              const int32_t* meta_hdr, const int32_t* meta, float scale, void* stream) {
+extern "C" int bsp_cache_attn_rows(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D, int64_t q_sz, int64_t q_sh,
+                                   int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st, const void* data, int num_pages, int page,
+                                   const int32_t* pages, int64_t pages_sz, int slots, const int32_t* lengths, int block,
+                                   const int32_t* meta_hdr, const int32_t* meta, int rows, float scale, void* stream) {
   using namespace bsp;
   if (dtype != BSP_F16 && dtype != BSP_BF16) return fail(BSP_ERR_INVALID, "cache attention: queries must be FP16 or BF16");
   if (Z < 0 || T < 0 || Hk < 1 || Hq < 0 || num_pages < 0 || slots < 0) return fail(BSP_ERR_INVALID, "cache attention: bad sizes (Z %d, heads %d over %d, T %d)", Z, Hq, Hk, T);
@@ -683,6 +683,7 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   if (meta_hdr[0] != BSP_META_MAGIC) return fail(BSP_ERR_INVALID, "cache attention: bad layout header (magic)");
   if (meta_hdr[2] != meta_hdr[3]) return fail(BSP_ERR_INVALID, "cache attention: the layout is not square");
   if (meta_hdr[1] != 1 && meta_hdr[1] != Hk) return fail(BSP_ERR_INVALID, "cache attention: layout of %d heads for a cache of %d", meta_hdr[1], Hk);
+  if (rows < 0 || rows > meta_hdr[2]) return fail(BSP_ERR_INVALID, "cache attention: %d rows of a layout of %d", rows, meta_hdr[2]);
   if (static_cast<int64_t>(meta_hdr[2]) * block > INT32_MAX) return fail(BSP_ERR_UNSUPPORTED, "cache attention: sequences of up to 2^31 tokens");
   if (Z == 0 || T == 0 || Hq == 0) return BSP_OK;
   if (!q || !o || !lengths || (slots && !pages) || (num_pages && !data)) return fail(BSP_ERR_INVALID, "cache attention: NULL argument");
@@ -701,7 +702,7 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   p.pages = {pages, pages_sz, slots, num_pages, Hk, log2_of(page / kGranule)};
   p.lengths = lengths;
   p.row_ptr = mt.row_ptr; p.blk_col = mt.blk_col;
-  p.layout_heads = mt.H; p.layout_rows = mt.Mb; p.block_shift = log2_of(block / kGranule);
+  p.layout_heads = mt.H; p.layout_rows = mt.Mb; p.rows = rows; p.block_shift = log2_of(block / kGranule);
   p.T = T; p.G = Hq / Hk;
   if (static_cast<int64_t>(T) * p.G > INT32_MAX / 2) return fail(BSP_ERR_UNSUPPORTED, "cache attention: too many queries");
   p.tiles = (T * p.G + kQueries - 1) / kQueries;
@@ -719,4 +720,12 @@ extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, 
   const int queries = T * p.G;
   if (dtype == BSP_F16) return D == 64 ? pick<__half, 64>(p, groups, queries, many, s) : pick<__half, 128>(p, groups, queries, many, s);
   return D == 64 ? pick<__nv_bfloat16, 64>(p, groups, queries, many, s) : pick<__nv_bfloat16, 128>(p, groups, queries, many, s);
+}
+
+extern "C" int bsp_cache_attn(const void* q, void* o, int dtype, int Z, int Hq, int Hk, int T, int D, int64_t q_sz, int64_t q_sh,
+                              int64_t q_st, int64_t o_sz, int64_t o_sh, int64_t o_st, const void* data, int num_pages, int page,
+                              const int32_t* pages, int64_t pages_sz, int slots, const int32_t* lengths, int block,
+                              const int32_t* meta_hdr, const int32_t* meta, float scale, void* stream) {
+  return bsp_cache_attn_rows(q, o, dtype, Z, Hq, Hk, T, D, q_sz, q_sh, q_st, o_sz, o_sh, o_st, data, num_pages, page, pages, pages_sz, slots,
+                             lengths, block, meta_hdr, meta, meta_hdr ? meta_hdr[2] : 0, scale, stream);
 }

@@ -215,7 +215,7 @@ std::pair<Tensor, Tensor> cache_read(const c10::intrusive_ptr<CacheOp>& c, const
 // ---- attention over the cache --------------------------------------------------------------------
 struct CacheAttentionOp : torch::CustomClassHolder {
   Tensor hdr, meta;                        // header (host) and tables (device) of the layout
-  int64_t block;
+  int64_t block, rows;                     // rows: those of the layout that count
 };
 
 Tensor cache_attention(const c10::intrusive_ptr<CacheAttentionOp>& p, const Tensor& q0, const c10::intrusive_ptr<CacheOp>& c,
@@ -230,10 +230,10 @@ Tensor cache_attention(const c10::intrusive_ptr<CacheAttentionOp>& p, const Tens
   const Tensor q = even_rows(q0, true), o = at::empty(q.sizes(), q.options());
   const int64_t Z = q.size(0);
   const PageTable t = page_table(pages, Z, *c);
-  check(bsp_cache_attn(q.const_data_ptr(), o.mutable_data_ptr(), code, Z, q.size(1), c->heads(), q.size(2), c->head_dim, q.stride(0),
+  check(bsp_cache_attn_rows(q.const_data_ptr(), o.mutable_data_ptr(), code, Z, q.size(1), c->heads(), q.size(2), c->head_dim, q.stride(0),
                        q.stride(1), q.stride(2), o.stride(0), o.stride(1), o.stride(2), c->data.const_data_ptr(), c->pages(), c->page,
                        t.at, t.stride, t.slots, per_sequence(lengths, Z, *c, "lengths"), p->block, p->hdr.const_data_ptr<int32_t>(),
-                       p->meta.const_data_ptr<int32_t>(), static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(c->head_dim))), stream_of(q)));
+                       p->meta.const_data_ptr<int32_t>(), static_cast<int>(p->rows), static_cast<float>(scale ? *scale : 1.0 / std::sqrt(static_cast<double>(c->head_dim))), stream_of(q)));
   return o;
 }
 
@@ -260,9 +260,9 @@ void bind_serving(pybind11::module_& m) {
       .def("write", &cache_write, py::call_guard<py::gil_scoped_release>())
       .def("read", &cache_read, py::call_guard<py::gil_scoped_release>());
   py::class_<CacheAttentionOp, c10::intrusive_ptr<CacheAttentionOp>>(m, "CacheAttentionOp")
-      .def(py::init([](Tensor hdr, Tensor meta, int64_t block) {
+      .def(py::init([](Tensor hdr, Tensor meta, int64_t block, int64_t rows) {
         auto p = c10::make_intrusive<CacheAttentionOp>();
-        p->hdr = hdr; p->meta = meta; p->block = block;
+        p->hdr = hdr; p->meta = meta; p->block = block; p->rows = rows;
         return p;
       }))
       .def("__call__", &cache_attention, py::call_guard<py::gil_scoped_release>());
