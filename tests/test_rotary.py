@@ -147,6 +147,45 @@ def test_gradient_is_the_turn_back(dtype, interleaved):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('tracked', ['q', 'k'])
+def test_an_operand_that_needs_no_gradient(tracked):
+    """Its result needs none either, and none is turned back for it, also where both results are used."""
+    rotary = Rotary(16, (4, 4))
+    positions = torch.randint(0, 50, (2, 5), device='cuda')
+    x = {n: operand((1, 2, 5, 16), torch.float32, seed=i) for i, n in enumerate('qk')}
+    x[tracked].requires_grad_()
+    y = dict(zip('qk', rotary(x['q'], x['k'], positions)))
+    other = 'k' if tracked == 'q' else 'q'
+    assert y[tracked].requires_grad and not y[other].requires_grad and y[other].grad_fn is None
+    assert torch.equal(y[other], rotary(x[other], positions=positions))
+    d = operand((1, 2, 5, 16), torch.float32, seed=5)
+    g, = torch.autograd.grad((y[tracked] * y[other].cos()).sum() + (y[tracked] * d).sum(), x[tracked])
+    assert_turned(g, rotary, d + y[other].cos(), positions, -1)
+    # differentiated again with respect to one incoming gradient of two
+    z = {n: t.detach().requires_grad_() for n, t in x.items()}
+    w = {n: d.clone().requires_grad_(n == tracked) for n in 'qk'}
+    yq, yk = rotary(z['q'], z['k'], positions)
+    g = dict(zip('qk', torch.autograd.grad((yq, yk), (z['q'], z['k']), (w['q'], w['k']), create_graph=True)))
+    assert g[tracked].requires_grad and not g[other].requires_grad
+    gg, = torch.autograd.grad(g[tracked], w[tracked], d)
+    assert_turned(gg, rotary, d, positions)
+
+
+@pytest.mark.gpu
+def test_tangents_and_batched_transforms_are_refused():
+    """Passing them by would drop a derivative without a word."""
+    import torch.autograd.forward_ad as fwad
+    rotary, x, t = Rotary(16), operand((1, 2, 5, 16), torch.float32), operand((1, 2, 5, 16), torch.float32, seed=1)
+    with fwad.dual_level():
+        dual = fwad.make_dual(x, t)
+        for args in ((dual,), (dual, x), (x, dual), (x.clone().requires_grad_(), dual)):
+            with pytest.raises(RuntimeError, match='jvp'):
+                rotary(*args)
+    with pytest.raises(RuntimeError):
+        torch.func.vmap(rotary)(torch.stack([x, t]))
+
+
+@pytest.mark.gpu
 def test_gradient_against_differences_and_again():
     rotary = Rotary(16, (4, 4))
     positions = torch.randint(0, 50, (2, 5), device='cuda')

@@ -96,6 +96,8 @@ struct RotaryFn : torch::autograd::Function<RotaryFn> {
     ctx->saved_data["q"] = q.has_value();
     if (pos) ctx->save_for_backward({*pos});
     auto [yq, yk] = rotary(*p, q, k, pos, inverse);
+    // (an operand that needs no gradient: its result needs none either, and the backward does not turn one for it)
+    if (q && k && needs_grad(*q) != needs_grad(*k)) ctx->mark_non_differentiable({needs_grad(*q) ? yk : yq});
     if (!q) return {yk};
     return k ? variable_list{yq, yk} : variable_list{yq};
   }
