@@ -114,6 +114,27 @@ def test_far_and_negative_positions(kind):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize('interleaved', [False, True])
+def test_small_sines_and_cosines_keep_their_bits(interleaved):
+    """Angles next to whole quarters of a turn, turning (1, 0): the result is the cosine and the sine alone.
+
+    sincospif is off by at most 2 ulp (2^-22), its argument by 2^-24 of itself, which at most an eighth of a turn
+    away from a quarter is 1.1 * 2^-24 of the sine and less of the cosine: below 2^-21 together.  The table's rounding
+    adds |position| * 2^-62, the oracle's product of doubles 2^-52 of the angle."""
+    near = [k * math.pi / 2 + s * d for k in range(-4, 5) for d in (2.0 ** -20, 1e-4, 0.03) for s in (1, -1)]
+    rotary = Rotary(2 * len(near), frequencies=near, interleaved=interleaved)
+    positions = torch.tensor([1, -1, 5, 1001], device='cuda')
+    x = torch.zeros((1, 1, 4, 2 * len(near)), device='cuda')
+    first, second = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, len(near)), slice(len(near), None))
+    x[..., first] = 1
+    y = rotary(x, positions=positions)[0, 0].double().cpu()
+    angle = positions.double().cpu()[:, None] * torch.tensor(near, dtype=torch.float64)
+    for got, want in ((y[:, first], angle.cos()), (y[:, second], angle.sin())):
+        limit = want.abs() * 2.0 ** -21 + positions.cpu().abs()[:, None] * 2.0 ** -62 + angle.abs() * 2.0 ** -52
+        assert bool(((got - want).abs() <= limit).all()), ((got - want).abs() / limit).max()
+
+
+@pytest.mark.gpu
 def test_given_frequencies_and_default_positions():
     rotary = Rotary(32, (5, 4), frequencies=[0.0, 1.0, 3.5, -2.0, 1e-9, 6.2, 0.5, 0.25, 7.0])
     positions = torch.arange(2 * 3 * 11, device='cuda').view(2, 3, 11)

@@ -8,8 +8,10 @@
 // Angles.  A float loses the angle of a far position (2^20 times a frequency near 1 is off by up to
 // 2^-5 rad), and doubles are slow.  The table holds each frequency as a 64-bit fraction of a whole
 // turn, F = round(freq / 2 pi * 2^64); position * F modulo 2^64 is then the exact fraction of a turn of
-// F (two's complement, so negative positions turn back), and its leading bits, as a float in [-1, 1)
-// half turns, go to sincospif.  The float's rounding (2^-25 of half a turn: 9e-8 rad) is what remains.
+// F (two's complement, so negative positions turn back).  Whole quarters of a turn are taken off it as integers, the rest,
+// an eighth of a turn at most, goes to sincospif as a float, and the quarters come back as exchanges and signs.  So the float's
+// rounding, 2^-24 of the rest, is no more than the last place of either result (as a float of up to half a turn the angle
+// alone would be off by 9e-8 rad).
 //
 // Bound by memory: every element is read once and written once.  A CTA takes up to 8 tokens of all heads of
 // q and k, computes the sines of its tokens once into shared memory (a pair's sine serves every
@@ -107,9 +109,19 @@ __global__ void __launch_bounds__(kThreads, VEC == 8 && !INTER ? 5 : 4) rotary_k
       const int64_t at = axis * p.p_sa + zn * p.p_sz + ln * p.p_sl;
       pos = p.pos_bytes == 4 ? static_cast<const int32_t*>(p.positions)[at] : static_cast<const int64_t*>(p.positions)[at];
     }
-    const int64_t turn = static_cast<int64_t>(static_cast<uint64_t>(pos) * static_cast<uint64_t>(p.table[pr]));
+    const uint64_t turn = static_cast<uint64_t>(pos) * static_cast<uint64_t>(p.table[pr]);
+    const uint32_t quarters = static_cast<uint32_t>((turn + (1ull << 61)) >> 62);
     float s, c;
-    sincospif(__ll2float_rn(turn) * 0x1p-63f, &s, &c);
+    sincospif(__ll2float_rn(static_cast<int64_t>(turn - (static_cast<uint64_t>(quarters) << 62))) * 0x1p-63f, &s, &c);
+    if (quarters & 1) {
+      const float t = s;
+      s = c;
+      c = -t;
+    }
+    if (quarters & 2) {
+      s = -s;
+      c = -c;
+    }
     cs[i] = make_float2(c, p.inverse ? -s : s);
   }
   __syncthreads();

@@ -29,8 +29,9 @@ class Rotary(_lib.WithOps):
     or BF16; any strides; the numbers of heads may differ) and returns the turned query, or query and
     key, as new tensors in their operands' memory order.  positions: int32 or int64 on the same device,
     [axes, L] or [axes, Z, L], or [L] for one axis, negative ones too; None: 0, 1, .. L - 1 on one axis.
-    Angles are exact to 2^-25 of a half turn at any position.  (The first call on a device uploads a table: not inside a capture.)  Both operands are differentiable (the
-    gradient is turned back), positions are not.
+    Angles are off by at most |position| * 2^-62 radians, sines and cosines beyond that by 2^-21 of themselves.
+    Both operands are differentiable (the gradient is turned back), positions are not.  The first call on a
+    device uploads a table: not inside a capture.
     """
 
     _op_attributes = frozenset(('head_dim', 'sections', 'base', 'interleaved', 'frequencies'))
