@@ -313,6 +313,16 @@ def test_traced():
 
 
 @pytest.mark.gpu
+def test_a_trace_refuses_what_a_call_refuses():
+    rotary, q = Rotary(32), operand((2, 3, 6, 32), torch.float16)
+    for k in (q.float(), q[:, :, :5], q[:1], q[..., :30]):
+        with pytest.raises(ValueError):
+            rotary(q, k)
+        with pytest.raises(ValueError):
+            torch.jit.trace(lambda a, b: rotary(a, b), (q, k), check_trace=False)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize('train', [False, True])
 def test_multihead_attention_with_positions(train):
     L, B, E, H = 64, 2, 128, 2

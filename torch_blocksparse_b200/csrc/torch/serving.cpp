@@ -136,8 +136,7 @@ void check_rotary(const RotaryOp& p, const Tensor& x, const char* what) {
   TORCH_CHECK(x.device() == p.table.device(), "rotary: ", what, " is on ", x.device(), ", the call runs on ", p.table.device());
 }
 
-std::pair<Tensor, OptTensor> rotary_call(const c10::intrusive_ptr<RotaryOp>& p, const Tensor& q, const OptTensor& k,
-                                         const OptTensor& pos) {
+void check_rotary_call(const c10::intrusive_ptr<RotaryOp>& p, const Tensor& q, const OptTensor& k) {
   check_rotary(*p, q, "the query");
   if (k) {
     check_rotary(*p, *k, "the key");
@@ -145,6 +144,11 @@ std::pair<Tensor, OptTensor> rotary_call(const c10::intrusive_ptr<RotaryOp>& p, 
     TORCH_CHECK_VALUE(k->size(0) == q.size(0) && k->size(2) == q.size(2), "rotary: query ", q.sizes(), " and key ", k->sizes(),
                       " differ in batch or length");
   }
+}
+
+std::pair<Tensor, OptTensor> rotary_call(const c10::intrusive_ptr<RotaryOp>& p, const Tensor& q, const OptTensor& k,
+                                         const OptTensor& pos) {
+  check_rotary_call(p, q, k);
   auto [yq, yk] = rotary_recorded(p, q, k, pos, false);
   return {yq, yk.defined() ? OptTensor(yk) : OptTensor()};
 }
@@ -250,6 +254,7 @@ void bind_serving(pybind11::module_& m) {
         return p;
       }))
       .def("__call__", &rotary_call, py::call_guard<py::gil_scoped_release>())
+      .def("check", &check_rotary_call, py::call_guard<py::gil_scoped_release>())
       .def("one", [](const c10::intrusive_ptr<RotaryOp>& p, const Tensor& x, const OptTensor& pos) { return rotary_call(p, x, {}, pos).first; },
            py::call_guard<py::gil_scoped_release>());
   py::class_<CacheOp, c10::intrusive_ptr<CacheOp>>(m, "CacheOp")

@@ -74,6 +74,7 @@ class Rotary(_lib.WithOps):
             raise RuntimeError(f'torch_blocksparse_b200 runs on CUDA tensors only (got a {query.device} tensor)')
         op = self._ops.get(query.get_device()) or self._op(query.device)
         if recording() is not None:
+            op.check(query, key)
             q = tracing.call(op, 'one', query, positions)
             return q if key is None else (q, tracing.call(op, 'one', key, positions))
         q, k = op(query, key, positions)
