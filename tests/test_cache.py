@@ -302,3 +302,13 @@ def test_bad_calls():
     cache.data = cache.data[:, :1]
     with pytest.raises(ValueError, match='contiguous'):
         cache.read(pages, start, 5)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_an_int_counts_are_refused():
+    """An operand whose rows share memory can be as long; none of it is written."""
+    cache, pages = KVCache(2, 1, 64, page=16), ints(0, 1)[None]
+    x = tokens(1, 1, 1, 64, torch.float16).expand(1, 1, 2 ** 32 + 5, 64)
+    with pytest.raises(NotImplementedError):
+        cache.write(x, x, pages, ints(0))
+    assert not bool(cache.data.any())

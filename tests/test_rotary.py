@@ -415,3 +415,11 @@ def test_bad_calls():
         rotary(q, positions=positions.cpu())
     with pytest.raises(RuntimeError):
         rotary(q, q.cpu(), positions)
+
+
+@pytest.mark.gpu
+def test_more_tokens_than_an_int_counts_are_refused():
+    x = torch.zeros((1, 1, 1, 2), device='cuda', dtype=torch.float16)
+    for shape in ((1, 1, 2 ** 32 + 5, 2), (2 ** 32 + 5, 1, 1, 2), (1, 2 ** 32 + 5, 1, 2)):
+        with pytest.raises(NotImplementedError):
+            Rotary(2)(x.expand(shape))

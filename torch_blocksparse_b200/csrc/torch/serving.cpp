@@ -133,6 +133,7 @@ void check_rotary(const RotaryOp& p, const Tensor& x, const char* what) {
   TORCH_CHECK_VALUE(x.dim() == 4 && x.size(3) == p.head_dim, "rotary: ", what, " must be [Z, H, L, ", p.head_dim, "] (got ", x.sizes(), ")");
   require_cuda(x);
   dtype_code(x);
+  TORCH_CHECK_NOT_IMPLEMENTED(x.size(0) <= INT32_MAX && x.size(1) <= INT32_MAX && x.size(2) <= INT32_MAX, "rotary: too many tokens ", x.sizes());
   TORCH_CHECK(x.device() == p.table.device(), "rotary: ", what, " is on ", x.device(), ", the call runs on ", p.table.device());
 }
 
@@ -174,6 +175,7 @@ struct PageTable {
   int64_t stride, slots;
 };
 PageTable page_table(const Tensor& t, int64_t Z, const CacheOp& c) {
+  TORCH_CHECK_NOT_IMPLEMENTED(t.dim() != 2 || t.size(1) * c.page <= INT32_MAX, "sequences of up to 2^31 tokens (got a table of ", t.sizes(), " pages)");
   TORCH_CHECK(t.device() == c.data.device(), "the page table is on ", t.device(), ", the cache on ", c.data.device());
   TORCH_CHECK_VALUE(t.scalar_type() == at::kInt && t.dim() == 2 && t.size(0) == Z && (t.size(1) < 2 || t.stride(1) == 1),
                     "pages must be int32 [", Z, ", slots] with unit stride on the slots (got ", t.scalar_type(), " ", t.sizes(), ")");
@@ -192,6 +194,8 @@ void cache_write(const c10::intrusive_ptr<CacheOp>& c, const Tensor& k0, const T
   require_cuda(k0);
   TORCH_CHECK(k0.device() == c->data.device(), "the key is on ", k0.device(), ", the cache on ", c->data.device());
   require_same(v0, k0, "the value");
+  // (rows of a tensor may share memory, so that there can be more than an int counts)
+  TORCH_CHECK_NOT_IMPLEMENTED(k0.size(0) <= INT32_MAX && k0.size(2) <= INT32_MAX, "cannot write ", k0.sizes(), " tokens at once");
   const int code = dtype_code(k0);
   no_gradient(k0, "the key");
   no_gradient(v0, "the value");
