@@ -58,6 +58,7 @@ namespace cg = cooperative_groups;
 constexpr int kWarps = 4;
 constexpr int kStages = 2;
 constexpr int kCtas = 4;            // on an SM
+constexpr int kSms = 148;
 constexpr int kQueries = 8;
 constexpr int kMaxCluster = 8;
 constexpr float kNothing = -3e38f; // the maximum of no scores
@@ -713,7 +714,7 @@ extern "C" int bsp_cache_attn_rows(const void* q, void* o, int dtype, int Z, int
   // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys, eight
   // queries each: 107 us, one at a time 119); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 11.3 us, one at a time 9.9).
   const int64_t granules = (static_cast<int64_t>(mt.nnz) / std::max<int64_t>(1, static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
-  p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * 148 / groups, granules / kWarps})));
+  p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * kSms / groups, granules / kWarps})));
   const bool many = granules > 16 * kWarps * p.cluster;
   if (Z > INT32_MAX / Hk / p.tiles / p.cluster) return fail(BSP_ERR_UNSUPPORTED, "cache attention: too many queries");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
