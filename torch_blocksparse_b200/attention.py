@@ -231,7 +231,8 @@ class DeepSpeedSparseSelfAttention(_lib.WithOps, nn.Module):
         the nonzero blocks of its block-row: what forward() gives for that row under a causal
         attn_mask.  The layout is the module's own, [heads of the cache or 1, ...], or its configuration's for
         sequences as long as the page table; rows behind its end see nothing.  Positions below zero
-        (sequences shorter than T) and queries that see nothing give zeros.  scale: head_dim ** -0.5;
+        (sequences shorter than T) and queries that see nothing give zeros.  scale: head_dim ** -0.5
+        (1.0 for queries that are scaled already, as MultiheadAttention scales them in front of its `core`);
         where scale times a query's largest channel is above 2 ** 119 its result is NaN.
 
         One kernel, without workspace, on the current stream of the cache's device; no gradient.  Lengths

@@ -34,11 +34,13 @@
 // once, in shared memory, then by sending them over the cluster, in a fixed order: results do not depend on timing.
 //
 // What bounds it now.  592 heads x 8192 keys, all of a layout, bf16: 128 channels, one query each 111 us, 96 % of the copy rate, four
-// 121 us, 88 %, eight 140 us, 77 %; 64 channels 70 us, 76 % (fp16: 85, 75 and 67 % with one, four, and one of 64).  Short of the memory's
-// rate it is instructions: masks, permutations, packing and maxima hold an SM's issue ports two cycles each (for 16 tokens of 128
-// channels and eight queries 64 + 16 + 8 + 8 of them), a product of 16 x 8 x 16 the tensor pipe 8.3 and the port two, everything else one:
-// 490 cycles of an SM's quarter where loading takes 375.  More warps an SM (96 or 80 registers) change nothing.  Short rows are bound by
-// the chain of loads (length, row, block, page, data), the launch and the join: 5 us for 5 granules a warp.
+// 122 us, 87 %, eight 146 us, 73 %; 64 channels, up to four queries 71 us, 75 %, eight 84, 64 % (fp16: 126, 144 and 182 us, 85, 74 and 59 %; 81 and
+// 99 us, 66 and 54 %).  Short of the memory's rate it is instructions: masks, permutations, packing and maxima hold an SM's issue
+// ports two cycles each (for 16 tokens of 128 channels and eight queries 64 + 16 + 8 + 8 of them), a product of 16 x 8 x 16 the tensor pipe
+// 8.3 and the port two, everything else one: 510 cycles of an SM's quarter where loading takes 375.  More warps an SM (96 or 80 registers)
+// change nothing.  Short rows are bound by the chain of loads (length, row, block, page, data), the launch and the join: 4.8 us for 5
+// granules a warp.  More than eight queries take the granules again for every eight (16 x 8 heads of 32768 keys, bf16, 128 channels: 8, 16, 32 and
+// 128 queries 150, 283, 542 and 1818 us).
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -658,7 +660,7 @@ template <typename T, int D, int GC> int pick(const AttnParams& p, int64_t group
   return many ? launch<T, D, GC, 256 / D>(p, groups, stream) : launch<T, D, GC, 1>(p, groups, stream);
 }
 // As many groups of channels beside the queries in the products' columns as there are places (592 heads x 8192 keys of 128,
-// bf16: one query with 4 groups 111 us, with 2 120, with 1 138; four queries with 2 groups 121, with 1 138).
+// bf16: one query with 4 groups 111 us, with 2 120, with 1 140; four queries with 2 groups 122, with 1 143).
 template <typename T, int D> int pick(const AttnParams& p, int64_t groups, int queries, bool many, cudaStream_t stream) {
   if constexpr (D == 128)
     if (queries <= 2) return pick<T, D, 4>(p, groups, many, stream);
@@ -709,10 +711,10 @@ extern "C" int bsp_cache_attn_rows(const void* q, void* o, int dtype, int Z, int
   p.tiles = (T * p.G + kQueries - 1) / kQueries;
   p.scale_log2e = scale * 1.4426950408889634f;
   const int64_t groups = static_cast<int64_t>(Z) * Hk * p.tiles;
-  // CTAs of a cluster: as many as fit the SMs at once (one sequence of 12 heads, rows of up to 19 blocks of 64: 8 CTAs 5.0 us,
-  // one 6.4; 8 x 16 heads, 36 blocks: 4 CTAs 9.9 us, one 16.3, 8 CTAs, which do not fit, 14.6), and a granule of an average row
-  // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (16 x 8 heads of 32768 keys, eight
-  // queries each: 107 us, one at a time 119); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 11.3 us, one at a time 9.9).
+  // CTAs of a cluster: as many as fit the SMs at once (one sequence of 12 heads, rows of up to 19 blocks of 64: 8 CTAs 4.8 us,
+  // one 5.8; 8 x 16 heads, 36 blocks: 4 CTAs 9.7 us, one 14.9, 8 CTAs, which do not fit, 14.4), and a granule of an average row
+  // for every warp.  Two granules of 128 or four of 64 channels at a time where a warp has many (592 heads x 8192 keys of 128, one and eight
+  // queries: 111 and 146 us, one at a time 120 and 160); fewer fill such steps badly (the 8 x 16 heads above, 9 granules a warp: 11.5 us, one at a time 9.7).
   const int64_t granules = (static_cast<int64_t>(mt.nnz) / std::max<int64_t>(1, static_cast<int64_t>(mt.H) * mt.Mb) + 1) << p.block_shift;
   p.cluster = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>({kMaxCluster, kCtas * kSms / groups, granules / kWarps})));
   const bool many = granules > 16 * kWarps * p.cluster;
